@@ -152,6 +152,159 @@ int sj_gemm_e4m3(const uint8_t* A, const uint8_t* W, const float* sa, const floa
                  int geglu, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* 1b. Operators of an encoder layer (device pointers, async on `stream`).   */
+/*                                                                           */
+/* Masked and biased attention, a projection with a low-rank adapter for each */
+/* request, and the step of norms, gate and residual between two blocks.  No  */
+/* counterpart in the reference.  Conventions as above: caller-owned device   */
+/* memory, a status and a message, nothing allocated.  What depends on a      */
+/* batch's lengths alone (which keys a tile of queries needs, which adapters  */
+/* a tile of rows needs) is worked out once per batch on the host by a        */
+/* *_plan function into memory of the caller, who copies it to the device and */
+/* uses it in every layer.  A plan function called with plan == NULL only     */
+/* fills `info` (info->plan_len says how many int32 the plan takes).          */
+/* ------------------------------------------------------------------------- */
+
+/* Which keys each query row of a packed batch sees.  Segment b = rows
+ * [cu_seqlens[b], cu_seqlens[b+1]); documents are a finer partition of the
+ * rows.  Query row i sees key row j of its segment (jr = j - cu_seqlens[b]) iff
+ *   jr < kv_lens[b] and
+ *   (jr < prefix[b] or (j in i's document, and j <= i when causal,
+ *                       and |i - j| <= window when window > 0)).
+ * All arrays are host memory; NULL docs: a segment is one document, NULL
+ * prefix: none, NULL kv_lens: the whole segment, NULL q_rows: every row asks.
+ * With q_rows (strictly increasing packed row numbers) only those rows ask,
+ * and q and O have a row for each of them. */
+typedef struct sj_attn_plan_args {
+  const int32_t* cu_seqlens; /* [B + 1], starts at 0, non-decreasing */
+  int B;
+  const int32_t* docs;       /* [n_docs + 1] row boundaries; every segment boundary is one */
+  int n_docs;
+  const int32_t* prefix;     /* [B], 0 .. length */
+  const int32_t* kv_lens;    /* [B], >= 0 (clipped to the length) */
+  const int32_t* q_rows;     /* [n_q] */
+  int n_q;
+  int causal;
+  int window;                /* >= 0; 0: none */
+} sj_attn_plan_args;
+
+typedef struct sj_attn_plan_info {
+  int64_t plan_len;  /* int32 words */
+  int32_t n_rows;    /* query rows */
+  int32_t n_keys;    /* key rows */
+  int32_t n_items;   /* tiles of up to 128 query rows */
+  int32_t n_tiles;   /* 64-key tiles over all items */
+  int64_t off_items, off_tiles; /* word offsets into the plan */
+} sj_attn_plan_info;
+
+int sj_attn_plan(const sj_attn_plan_args* args, int32_t* plan, int64_t plan_len,
+                 sj_attn_plan_info* info);
+
+/* O = softmax over the visible keys of
+ *   x = scale q.k;  x = softcap tanh(x / softcap) when softcap > 0;
+ *   x += rel_bias[h][clamp(j - i, -rel_max, rel_max) + rel_max] when rel_bias;
+ *   x -= slopes[h] |i - j| when slopes
+ * times V; a row that sees no key, or only keys with a score of -inf, gives 0,
+ * and what masked keys and values hold (NaN and infinities too) never reaches
+ * the output.
+ * q [n_rows, H, Dh], k and v [n_keys, Hkv, Dh], O [n_rows, H, Dh] bf16 with
+ * row pitches ldq, ldk, ldv, ldo in elements (q, k and v may be slices of one
+ * packed tensor); H % Hkv == 0, head h reads key head h / (H / Hkv);
+ * 1 <= Dh <= 128.  rel_bias fp32 [H, 2 rel_max + 1], slopes fp32 [H].
+ * plan: the device copy of sj_attn_plan's.  Scores, softmax statistics and
+ * sums are fp32. */
+typedef struct sj_attn_masked_args {
+  const sj_bf16 *q, *k, *v;
+  sj_bf16* O;
+  int64_t ldq, ldk, ldv, ldo;
+  int H, Hkv, Dh;
+  float scale;
+  float softcap;
+  const float* rel_bias;
+  int rel_max;
+  const float* slopes;
+} sj_attn_masked_args;
+
+/* Bytes of device workspace that sj_attn_masked needs (16-byte aligned; the
+ * caller's, one for each call in flight); -1 for a bad shape. */
+int64_t sj_attn_masked_workspace(const sj_attn_plan_info* info, int H, int Hkv, int Dh);
+
+int sj_attn_masked(const sj_attn_masked_args* args, const sj_attn_plan_info* info,
+                   const int32_t* plan, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Which low-rank adapter each packed row uses: segment b (host arrays, as
+ * above) uses adapter ids[b] in [0, n_adapters), or none (-1). */
+typedef struct sj_lora_plan_info {
+  int64_t plan_len;  /* int32 words */
+  int32_t M;         /* rows */
+  int32_t rank, n_adapters;
+  int32_t n_blocks;  /* blocks of 256 rows */
+  int32_t n_slabs;   /* (block, adapter, 16 of its ranks) */
+  int64_t off_blocks, off_slabs; /* word offsets into the plan */
+} sj_lora_plan_info;
+
+int sj_lora_plan(const int32_t* cu_seqlens_host, int B, const int32_t* ids, int n_adapters,
+                 int rank, int32_t* plan, int64_t plan_len, sj_lora_plan_info* info);
+
+/* C[M,N] = act(X W^T + bias + scale[a] (X A[a]^T) Bw[a]^T), a = the row's
+ * adapter (no such term for -1): X bf16 [M, K] with row pitch ldx, W bf16
+ * [N, K], A bf16 [n_adapters, rank, K], Bw bf16 [n_adapters, N, rank], scale
+ * fp32 [n_adapters] or NULL (1), bias fp32 [N] or NULL, act as sj_gemm, C bf16
+ * with row pitch ldc.  Sums are fp32; scale[a] X A[a]^T is rounded to bf16
+ * once on the way into the second product.  plan: the device copy. */
+typedef struct sj_gemm_lora_args {
+  const sj_bf16 *X, *W, *A, *Bw;
+  const float *scale, *bias;
+  sj_bf16* C;
+  int64_t ldx, ldc;
+  int N, K;
+  int act;
+} sj_gemm_lora_args;
+
+int64_t sj_gemm_lora_workspace(const sj_lora_plan_info* info, int N, int K);
+
+int sj_gemm_lora(const sj_gemm_lora_args* args, const sj_lora_plan_info* info,
+                 const int32_t* plan, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The step between two blocks:
+ *   z  = post_norm(r)           (r itself when post_w is NULL)
+ *   x' = alpha x + beta g z     (g: see gate_mode)
+ *   y  = pre_norm(x')           (skipped when y is NULL)
+ * for M rows of D.  post_norm and pre_norm are of `kind`, with weights and
+ * optional biases fp32 [D]; y is taken from x' before x' is rounded to x's
+ * type.  x_out may be x.  Types are SJ_TYPE_*; pitches are in elements.
+ * Statistics are fp32. */
+#define SJ_TYPE_F32 0
+#define SJ_TYPE_BF16 1
+#define SJ_NORM_LN 0   /* (v - mean) / sqrt(var + eps) */
+#define SJ_NORM_RMS 1  /* v / sqrt(mean(v^2) + eps) */
+#define SJ_GATE_NONE 0
+#define SJ_GATE_CHANNEL 1 /* fp32 [D] */
+#define SJ_GATE_SEGMENT 2 /* fp32 [n_segs, D], row i's segment from cu_seqlens (device) */
+#define SJ_GATE_ROW 3     /* sigmoid of gate [M, D] (gate_type, pitch ldg) */
+typedef struct sj_norm_block_args {
+  const void* x;
+  void* x_out;
+  const void* r;
+  void* y;
+  int x_type, r_type, y_type;
+  int64_t ldx, ldxo, ldr, ldy;
+  const float *post_w, *post_b, *pre_w, *pre_b;
+  int kind;
+  float eps;
+  const void* gate;
+  int gate_mode, gate_type;
+  int64_t ldg;
+  const int32_t* cu_seqlens;
+  int n_segs;
+  float alpha, beta;
+  int64_t M;
+  int D;
+} sj_norm_block_args;
+
+int sj_norm_block(const sj_norm_block_args* args, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* 2. Encoder engine (replaces FastSnapjudge, include/snapjudge/fast.hpp).    */
 /* ------------------------------------------------------------------------- */
 typedef struct sj_fast sj_fast;

@@ -28,7 +28,9 @@ SJ_ARCH_SJMODEL = 1
 # every symbol declared in include/snapjudge_b200.h
 EXPORTS = ["sj_b200_version", "sj_last_error", "sj_gemm", "sj_gemm_geglu", "sj_add_ln", "sj_rope",
            "sj_attn", "sj_attn_noalloc", "sj_check_device_errors", "sj_test_attn_wait_timeout",
-           "sj_quant_e4m3", "sj_gemm_e4m3", "sj_fast_create", "sj_fast_set_tensor", "sj_fast_set_heads",
+           "sj_quant_e4m3", "sj_gemm_e4m3", "sj_attn_plan", "sj_attn_masked_workspace",
+           "sj_attn_masked", "sj_lora_plan", "sj_gemm_lora_workspace", "sj_gemm_lora",
+           "sj_norm_block", "sj_fast_create", "sj_fast_set_tensor", "sj_fast_set_heads",
            "sj_fast_commit", "sj_fast_encode", "sj_fast_embed", "sj_fast_decide", "sj_fast_forward", "sj_fast_n_act",
            "sj_fast_encode_device",
            "sj_fast_sync", "sj_fast_launch_count", "sj_fast_set_profiling", "sj_fast_profile",
@@ -58,6 +60,45 @@ class FastConfig(C.Structure):
 _LIB = None
 _P = C.c_void_p
 _I = C.c_int
+_L = C.c_int64
+_F = C.c_float
+
+
+class AttnPlanArgs(C.Structure):
+    _fields_ = [("cu_seqlens", _P), ("B", _I), ("docs", _P), ("n_docs", _I), ("prefix", _P),
+                ("kv_lens", _P), ("q_rows", _P), ("n_q", _I), ("causal", _I), ("window", _I)]
+
+
+class AttnPlanInfo(C.Structure):
+    _fields_ = [("plan_len", _L), ("n_rows", C.c_int32), ("n_keys", C.c_int32),
+                ("n_items", C.c_int32), ("n_tiles", C.c_int32), ("off_items", _L),
+                ("off_tiles", _L)]
+
+
+class AttnMaskedArgs(C.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("O", _P), ("ldq", _L), ("ldk", _L),
+                ("ldv", _L), ("ldo", _L), ("H", _I), ("Hkv", _I), ("Dh", _I), ("scale", _F),
+                ("softcap", _F), ("rel_bias", _P), ("rel_max", _I), ("slopes", _P)]
+
+
+class LoraPlanInfo(C.Structure):
+    _fields_ = [("plan_len", _L), ("M", C.c_int32), ("rank", C.c_int32),
+                ("n_adapters", C.c_int32), ("n_blocks", C.c_int32), ("n_slabs", C.c_int32),
+                ("off_blocks", _L), ("off_slabs", _L)]
+
+
+class GemmLoraArgs(C.Structure):
+    _fields_ = [("X", _P), ("W", _P), ("A", _P), ("Bw", _P), ("scale", _P), ("bias", _P),
+                ("C", _P), ("ldx", _L), ("ldc", _L), ("N", _I), ("K", _I), ("act", _I)]
+
+
+class NormBlockArgs(C.Structure):
+    _fields_ = [("x", _P), ("x_out", _P), ("r", _P), ("y", _P), ("x_type", _I), ("r_type", _I),
+                ("y_type", _I), ("ldx", _L), ("ldxo", _L), ("ldr", _L), ("ldy", _L),
+                ("post_w", _P), ("post_b", _P), ("pre_w", _P), ("pre_b", _P), ("kind", _I),
+                ("eps", _F), ("gate", _P), ("gate_mode", _I), ("gate_type", _I), ("ldg", _L),
+                ("cu_seqlens", _P), ("n_segs", _I), ("alpha", _F), ("beta", _F), ("M", _L),
+                ("D", _I)]
 
 
 def lib() -> C.CDLL:
@@ -81,6 +122,17 @@ def lib() -> C.CDLL:
         L.sj_test_attn_wait_timeout.restype = None
         L.sj_quant_e4m3.argtypes = [_P, C.c_int64, _I, _P, _P, _P]
         L.sj_gemm_e4m3.argtypes = [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]
+        L.sj_attn_plan.argtypes = [C.POINTER(AttnPlanArgs), _P, _L, C.POINTER(AttnPlanInfo)]
+        L.sj_attn_masked_workspace.argtypes = [C.POINTER(AttnPlanInfo), _I, _I, _I]
+        L.sj_attn_masked_workspace.restype = _L
+        L.sj_attn_masked.argtypes = [C.POINTER(AttnMaskedArgs), C.POINTER(AttnPlanInfo), _P, _P,
+                                     _L, _P]
+        L.sj_lora_plan.argtypes = [_P, _I, _P, _I, _I, _P, _L, C.POINTER(LoraPlanInfo)]
+        L.sj_gemm_lora_workspace.argtypes = [C.POINTER(LoraPlanInfo), _I, _I]
+        L.sj_gemm_lora_workspace.restype = _L
+        L.sj_gemm_lora.argtypes = [C.POINTER(GemmLoraArgs), C.POINTER(LoraPlanInfo), _P, _P, _L,
+                                   _P]
+        L.sj_norm_block.argtypes = [C.POINTER(NormBlockArgs), _P]
         L.sj_fast_create.argtypes = [C.POINTER(FastConfig), C.POINTER(_P)]
         L.sj_fast_set_tensor.argtypes = [_P, C.c_char_p, _P, C.POINTER(C.c_int64), _I]
         L.sj_fast_set_heads.argtypes = [_P, _I, C.POINTER(_I), C.POINTER(_I)]

@@ -1,0 +1,113 @@
+// attn_masked.cuh — what the masked-attention kernels share: their parameters,
+// the score of a pair, and one row computed by one warp.
+#pragma once
+
+#include "../../include/snapjudge_b200.h"
+#include "common.cuh"
+
+namespace sjb {
+
+struct AttnMasked {
+  const bf16 *q, *k, *v;
+  bf16* O;
+  int64_t ldq, ldk, ldv, ldo;
+  int H, Hkv, Dh;
+  float scale, cap;           // cap 0: none
+  const float* rel_bias;      // [H, 2 rel_max + 1] or null
+  int rel_max;
+  const float* slopes;        // [H] or null
+  int n_rows, n_keys, n_items;
+  const int4* rows;           // plan: 2 x int4 for each query row
+  const int4* items;          // plan: one for each query tile
+  const int32_t* tiles;       // plan: key tiles
+};
+
+inline AttnMasked attn_masked_params(const sj_attn_masked_args& a, const sj_attn_plan_info& info,
+                                     const int32_t* plan) {
+  AttnMasked p{};
+  p.q = reinterpret_cast<const bf16*>(a.q);
+  p.k = reinterpret_cast<const bf16*>(a.k);
+  p.v = reinterpret_cast<const bf16*>(a.v);
+  p.O = reinterpret_cast<bf16*>(a.O);
+  p.ldq = a.ldq;
+  p.ldk = a.ldk;
+  p.ldv = a.ldv;
+  p.ldo = a.ldo;
+  p.H = a.H;
+  p.Hkv = a.Hkv;
+  p.Dh = a.Dh;
+  p.scale = a.scale;
+  p.cap = a.softcap;
+  p.rel_bias = a.rel_bias;
+  p.rel_max = a.rel_max;
+  p.slopes = a.slopes;
+  p.n_rows = info.n_rows;
+  p.n_keys = info.n_keys;
+  p.n_items = info.n_items;
+  p.rows = reinterpret_cast<const int4*>(plan);
+  p.items = reinterpret_cast<const int4*>(plan + info.off_items);
+  p.tiles = plan + info.off_tiles;
+  return p;
+}
+
+// The score of a pair at distance d = j - i; dot is q.k.
+__device__ __forceinline__ float attn_score(const AttnMasked& p, const float* rel, float slope,
+                                             float dot, int d) {
+  float x = dot * p.scale;
+  if (p.cap > 0.f) x = p.cap * tanhf(x / p.cap);
+  if (rel) x += rel[min(max(d, -p.rel_max), p.rel_max) + p.rel_max];
+  x -= slope * (float)abs(d);
+  return x;
+}
+
+// One query row of one head by one warp, online over 32 keys at a time; lane l
+// gets the output's dimensions l, l + 32, l + 64, l + 96 in o.
+__device__ __noinline__ void attn_masked_row(const AttnMasked& p, int row, int h, int lane,
+                                             float (&o)[4]) {
+  const int4 r0 = p.rows[2 * (int64_t)row], r1 = p.rows[2 * (int64_t)row + 1];
+  const int pos = r0.x, a0 = r0.y, na = r0.z - r0.y, b0 = r0.w, nk = na + (r1.x - r0.w);
+  const int hk = h / (p.H / p.Hkv);
+  const bf16* q = p.q + (int64_t)row * p.ldq + (int64_t)h * p.Dh;
+  const bf16* k = p.k + (int64_t)hk * p.Dh;
+  const bf16* v = p.v + (int64_t)hk * p.Dh;
+  const float* rel = p.rel_bias ? p.rel_bias + (int64_t)h * (2 * (int64_t)p.rel_max + 1) : nullptr;
+  const float slope = p.slopes ? p.slopes[h] : 0.f;
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) o[c] = 0.f;
+  for (int t = 0; t < nk; t += 32) {
+    const int e = t + lane;
+    const int j = e < na ? a0 + e : b0 + (e - na);
+    float x = -INFINITY;
+    if (e < nk) {
+      const bf16* kr = k + (int64_t)j * p.ldk;
+      float dot = 0.f;
+      for (int d = 0; d < p.Dh; ++d) dot += __bfloat162float(q[d]) * __bfloat162float(kr[d]);
+      x = attn_score(p, rel, slope, dot, j - pos);
+    }
+    const float mt = fmaxf(m, warp_max(x));
+    const float mu = mt == -INFINITY ? 0.f : mt;  // no finite score yet
+    const float f = expf(m - mu);
+    const float pr = e < nk ? expf(x - mu) : 0.f;
+    l = l * f + warp_sum(pr);
+    m = mt;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] *= f;
+    const int cnt = min(32, nk - t);
+    for (int s = 0; s < cnt; ++s) {
+      const float ps = __shfl_sync(0xffffffffu, pr, s);
+      const int js = __shfl_sync(0xffffffffu, j, s);
+      const bf16* vr = v + (int64_t)js * p.ldv;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (lane + 32 * c < p.Dh) o[c] += ps * __bfloat162float(vr[lane + 32 * c]);
+    }
+  }
+  // no visible key, or only scores of -inf: 0 (a NaN in l stays one)
+#pragma unroll
+  for (int c = 0; c < 4; ++c) o[c] = l == 0.f ? 0.f : o[c] / l;
+}
+
+cudaError_t attn_masked_simt(const AttnMasked& p, cudaStream_t st);
+
+}  // namespace sjb

@@ -52,7 +52,7 @@ void set_last_error(const std::string& m) { g_err = m; }
 
 extern "C" {
 
-int sj_b200_version(void) { return 100; }
+int sj_b200_version(void) { return 200; }
 
 const char* sj_last_error(void) { return g_err.c_str(); }
 

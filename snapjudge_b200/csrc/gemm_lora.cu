@@ -1,0 +1,150 @@
+// gemm_lora.cu — C = act(X W^T + bias + scale_a (X A_a^T) B_a^T), a = the row's
+// adapter: the entry point, and the kernels on CUDA cores that take every
+// shape and alignment.
+#include <algorithm>
+
+#include "gemm_lora.cuh"
+#include "kernels.h"
+
+namespace sjb {
+namespace {
+
+// U[row, r] = scale_a X[row] . A_a[r], rounded to bf16: one warp per (row, r)
+__global__ void __launch_bounds__(256) lora_shrink_simt(GemmLora p, bf16* __restrict__ U) {
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (w >= (int64_t)p.M * p.R) return;
+  const int row = (int)(w / p.R), r = (int)(w % p.R);
+  const int a = p.rows[row];
+  float s = 0.f;
+  if (a >= 0) {
+    const bf16* x = p.X + (int64_t)row * p.ldx;
+    const bf16* ar = p.A + ((int64_t)a * p.R + r) * p.K;
+    for (int k = lane; k < p.K; k += 32) s += __bfloat162float(x[k]) * __bfloat162float(ar[k]);
+    s = warp_sum(s) * (p.scale ? p.scale[a] : 1.f);
+  }
+  if (lane == 0) U[w] = __float2bfloat16(s);
+}
+
+// 64 x 64 output tile, 256 threads of 4 x 4, K and then R walked 16 at a time
+__global__ void __launch_bounds__(256) lora_gemm_simt(GemmLora p, const bf16* __restrict__ U) {
+  __shared__ float xs[16][65], ws[16][65];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int n0 = blockIdx.x * 64;
+  const int64_t m0 = (int64_t)blockIdx.y * 64;
+  float acc[4][4] = {};
+  for (int k0 = 0; k0 < p.K; k0 += 16) {
+    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
+      const int kk = e & 15, i = e >> 4, k = k0 + kk;
+      const int64_t m = m0 + i;
+      const int n = n0 + i;
+      xs[kk][i] = m < p.M && k < p.K ? __bfloat162float(p.X[m * p.ldx + k]) : 0.f;
+      ws[kk][i] = n < p.N && k < p.K ? __bfloat162float(p.W[(int64_t)n * p.K + k]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < 16; ++kk) {
+      float a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = xs[kk][ty + 16 * i], b[i] = ws[kk][tx + 16 * i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += a[i] * b[j];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + ty + 16 * i;
+    if (m >= p.M) continue;
+    const int a = p.rows[m];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + tx + 16 * j;
+      if (n >= p.N) continue;
+      float v = acc[i][j];
+      if (a >= 0) {
+        const bf16* u = U + m * p.R;
+        const bf16* b = p.B + ((int64_t)a * p.N + n) * p.R;
+        for (int r = 0; r < p.R; ++r) v += __bfloat162float(u[r]) * __bfloat162float(b[r]);
+      }
+      if (p.bias) v += p.bias[n];
+      if (p.act == ACT_GELU) v = gelu_erf(v);
+      else if (p.act == ACT_RELU) v = v < 0.f ? 0.f : v;  // a NaN stays one
+      p.C[m * p.ldc + n] = __float2bfloat16(v);
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t gemm_lora_simt(const GemmLora& p, void* U, cudaStream_t st) {
+  bf16* u = static_cast<bf16*>(U);
+  const int64_t blocks = ((int64_t)p.M * p.R + 7) / 8;
+  const int64_t mt = ((int64_t)p.M + 63) / 64;
+  if (blocks > 0x7fffffff || mt > 65535) return cudaErrorInvalidConfiguration;
+  lora_shrink_simt<<<(unsigned)blocks, 256, 0, st>>>(p, u);
+  lora_gemm_simt<<<dim3((p.N + 63) / 64, (unsigned)mt), 256, 0, st>>>(p, u);
+  return cudaGetLastError();
+}
+
+}  // namespace sjb
+
+namespace {
+int bad(const char* m) {
+  sjb::set_last_error(m);
+  return SJ_ERR_INVALID;
+}
+}  // namespace
+
+extern "C" {
+
+int64_t sj_gemm_lora_workspace(const sj_lora_plan_info* info, int N, int K) {
+  if (!info || N < 0 || K < 0) {
+    bad("bad projection shape");
+    return -1;
+  }
+  return (int64_t)info->M * info->rank * 2;
+}
+
+int sj_gemm_lora(const sj_gemm_lora_args* a, const sj_lora_plan_info* info, const int32_t* plan,
+                 void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!a || !info) return bad("null GEMM argument");
+  if (a->N < 0 || a->K < 0) return bad("negative GEMM size");
+  if (a->act < 0 || a->act > 2) return bad("act must be 0, 1 or 2");
+  if (info->M == 0 || a->N == 0) return SJ_OK;
+  if (a->ldx < a->K || a->ldc < a->N) return bad("a row pitch is smaller than its row");
+  if ((a->K && (!a->X || !a->W || (info->n_slabs && !a->A))) || (info->n_slabs && !a->Bw) || !a->C ||
+      !plan)
+    return bad("null GEMM operand");
+  const int64_t need = sj_gemm_lora_workspace(info, a->N, a->K);
+  if (workspace_bytes < need || (need > 0 && !workspace)) return bad("the workspace is too small");
+  sjb::GemmLora p{};
+  p.X = reinterpret_cast<const sjb::bf16*>(a->X);
+  p.W = reinterpret_cast<const sjb::bf16*>(a->W);
+  p.A = reinterpret_cast<const sjb::bf16*>(a->A);
+  p.B = reinterpret_cast<const sjb::bf16*>(a->Bw);
+  p.scale = a->scale;
+  p.bias = a->bias;
+  p.C = reinterpret_cast<sjb::bf16*>(a->C);
+  p.ldx = a->ldx;
+  p.ldc = a->ldc;
+  p.M = info->M;
+  p.N = a->N;
+  p.K = a->K;
+  p.R = info->rank;
+  p.act = a->act;
+  p.n_adapters = info->n_adapters;
+  p.n_blocks = info->n_blocks;
+  p.n_slabs = info->n_slabs;
+  p.rows = plan;
+  p.blocks = plan + info->off_blocks;
+  p.slabs = reinterpret_cast<const int2*>(plan + info->off_slabs);
+  const cudaError_t rc = sjb::gemm_lora_simt(p, workspace, static_cast<cudaStream_t>(stream));
+  if (rc == cudaSuccess) return SJ_OK;
+  sjb::set_last_error(std::string("snapjudge CUDA: gemm_lora: ") + cudaGetErrorString(rc));
+  return SJ_ERR_CUDA;
+}
+
+}  // extern "C"

@@ -1,0 +1,24 @@
+// gemm_lora.cuh — parameters of the projection with low-rank adapters.
+#pragma once
+
+#include "../../include/snapjudge_b200.h"
+#include "common.cuh"
+
+namespace sjb {
+
+struct GemmLora {
+  const bf16 *X, *W, *A, *B;  // [M, K], [N, K], [n_adapters, R, K], [n_adapters, N, R]
+  const float *scale, *bias;  // [n_adapters] or null, [N] or null
+  bf16* C;
+  int64_t ldx, ldc;
+  int M, N, K, R, act, n_adapters;
+  int n_blocks, n_slabs;
+  const int32_t* rows;    // plan: adapter of each row
+  const int32_t* blocks;  // plan: [n_blocks + 1]
+  const int2* slabs;      // plan: (adapter, sixteen)
+};
+
+// Kernels on CUDA cores for every shape and alignment; U: M x R bf16 of workspace.
+cudaError_t gemm_lora_simt(const GemmLora& p, void* U, cudaStream_t st);
+
+}  // namespace sjb

@@ -1,0 +1,349 @@
+// norm_block.cu — the step between two blocks: post-norm of a block's output,
+// gate, residual scale and add, and the next block's pre-norm, in one pass.
+//
+//   z  = post(r)                 post, pre: LN   (v - mean) / sqrt(var + eps) * w + b
+//   x' = alpha x + beta g z                 RMS  v / sqrt(mean(v^2) + eps) * w + b
+//   y  = pre(x')
+//
+// A row's x and r are read once, held in registers in fp32 (the statistics are
+// two-pass over them), and x' and y are written once: the bytes are x + r + x'
+// + y and the kernel is bound by HBM.  A row is held by a group of G threads,
+// NC chunks of VEC elements each: one warp for rows up to 1024 elements (no
+// barrier), a block of up to 1024 threads above; VEC = 4 where the width, the
+// pitches and the addresses allow it, else 1.  Rows too wide for that are read
+// once per statistic instead (norm_block_wide).
+#include <algorithm>
+
+#include "../../include/snapjudge_b200.h"
+#include "common.cuh"
+#include "kernels.h"
+
+namespace sjb {
+namespace {
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]);
+template <>
+__device__ __forceinline__ void load_vec<float, 1>(const float* p, float (&v)[1]) { v[0] = *p; }
+template <>
+__device__ __forceinline__ void load_vec<bf16, 1>(const bf16* p, float (&v)[1]) {
+  v[0] = __bfloat162float(*p);
+}
+template <>
+__device__ __forceinline__ void load_vec<float, 4>(const float* p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+}
+template <>
+__device__ __forceinline__ void load_vec<bf16, 4>(const bf16* p, float (&v)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]);
+template <>
+__device__ __forceinline__ void store_vec<float, 1>(float* p, const float (&v)[1]) { *p = v[0]; }
+template <>
+__device__ __forceinline__ void store_vec<bf16, 1>(bf16* p, const float (&v)[1]) {
+  *p = __float2bfloat16(v[0]);
+}
+template <>
+__device__ __forceinline__ void store_vec<float, 4>(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+template <>
+__device__ __forceinline__ void store_vec<bf16, 4>(bf16* p, const float (&v)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  uint2 u;
+  u.x = *reinterpret_cast<const uint32_t*>(&a);
+  u.y = *reinterpret_cast<const uint32_t*>(&b);
+  *reinterpret_cast<uint2*>(p) = u;
+}
+
+__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+
+// The segment that owns row r (largest b with cu[b] <= r), by a whole warp: 32
+// probes a step instead of a binary search's chain of dependent loads.
+__device__ __forceinline__ int warp_seg_of_row(const int32_t* cu, int B, int64_t r, int lane) {
+  int lo = 0, n = B;  // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int at = lo + lane * step;
+    const unsigned le = __ballot_sync(0xffffffffu, lane * step < n && cu[at] <= r);
+    const int hit = le ? 31 - __clz(le) : 0;  // cu is non-decreasing: a prefix of the lanes
+    n = min(step, n - hit * step);
+    lo += hit * step;
+  }
+  return lo;
+}
+
+// Sum over the group's threads; `red` has one float for each warp of the block
+// and is used for one sum only.
+template <bool WARP>
+__device__ __forceinline__ float group_sum(float v, float* red) {
+  v = warp_sum(v);
+  if (WARP) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  return warp_sum(lane < nw ? red[lane] : 0.f);
+}
+
+template <typename TX, typename TR, typename TY, int VEC, int NC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 1024)
+    norm_block_kernel(const sj_norm_block_args p) {
+  __shared__ float red[4][32];
+  const int lane = threadIdx.x & 31;
+  const int G = WARP ? 32 : (int)blockDim.x;
+  const int t = WARP ? lane : (int)threadIdx.x;
+  const int64_t row =
+      WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  if (row >= p.M) return;  // a whole group
+  const TX* x = static_cast<const TX*>(p.x) + row * p.ldx;
+  const TR* r = static_cast<const TR*>(p.r) + row * p.ldr;
+  const int nch = (p.D + VEC - 1) / VEC;  // VEC divides D
+  const float inv_d = 1.f / (float)p.D;
+
+  float xv[NC][VEC], zv[NC][VEC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int k = t + G * c;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) xv[c][e] = zv[c][e] = 0.f;
+    if (k < nch) {
+      load_vec<TX, VEC>(x + VEC * k, xv[c]);
+      load_vec<TR, VEC>(r + VEC * k, zv[c]);
+    }
+  }
+  int seg = 0;
+  if (p.gate_mode == SJ_GATE_SEGMENT) seg = warp_seg_of_row(p.cu_seqlens, p.n_segs, row, lane);
+
+  // v <- norm(v) before weight and bias; two-pass over the registers
+  auto normalise = [&](float (&v)[NC][VEC], float* red_mean, float* red_var) {
+    float mean = 0.f;
+    if (p.kind == SJ_NORM_LN) {
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s += v[c][e];
+      mean = group_sum<WARP>(s, red_mean) * inv_d;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (t + G * c < nch) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          v[c][e] -= mean;
+          q += v[c][e] * v[c][e];
+        }
+      }
+    const float inv = rsqrtf(group_sum<WARP>(q, red_var) * inv_d + p.eps);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[c][e] *= inv;
+  };
+  auto affine = [&](float (&v)[VEC], int k, const float* w, const float* b) {
+    float wv[VEC], bv[VEC];
+    load_vec<float, VEC>(w + VEC * k, wv);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] *= wv[e];
+    if (b) {
+      load_vec<float, VEC>(b + VEC * k, bv);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] += bv[e];
+    }
+  };
+
+  if (p.post_w) normalise(zv, red[0], red[1]);
+  TX* xo = static_cast<TX*>(p.x_out) + row * p.ldxo;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int k = t + G * c;
+    if (k >= nch) continue;
+    if (p.post_w) affine(zv[c], k, p.post_w, p.post_b);
+    if (p.gate_mode != SJ_GATE_NONE) {
+      float g[VEC];
+      if (p.gate_mode == SJ_GATE_ROW) {
+        if (p.gate_type == SJ_TYPE_BF16)
+          load_vec<bf16, VEC>(static_cast<const bf16*>(p.gate) + row * p.ldg + VEC * k, g);
+        else
+          load_vec<float, VEC>(static_cast<const float*>(p.gate) + row * p.ldg + VEC * k, g);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] = sigmoid(g[e]);
+      } else {
+        load_vec<float, VEC>(static_cast<const float*>(p.gate) + (int64_t)seg * p.D + VEC * k, g);
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) zv[c][e] *= g[e];
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) xv[c][e] = p.alpha * xv[c][e] + p.beta * zv[c][e];
+    store_vec<TX, VEC>(xo + VEC * k, xv[c]);
+  }
+  if (!p.y) return;
+  normalise(xv, red[2], red[3]);
+  TY* y = static_cast<TY*>(p.y) + row * p.ldy;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int k = t + G * c;
+    if (k >= nch) continue;
+    affine(xv[c], k, p.pre_w, p.pre_b);
+    store_vec<TY, VEC>(y + VEC * k, xv[c]);
+  }
+}
+
+// Rows wider than the registers of a block: every statistic reads the row again.
+template <typename TX, typename TR, typename TY>
+__global__ void __launch_bounds__(1024) norm_block_wide(const sj_norm_block_args p) {
+  __shared__ float red[4][32];
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x;
+  const TX* x = static_cast<const TX*>(p.x) + row * p.ldx;
+  const TR* r = static_cast<const TR*>(p.r) + row * p.ldr;
+  const float inv_d = 1.f / (float)p.D;
+  int seg = 0;
+  if (p.gate_mode == SJ_GATE_SEGMENT) seg = warp_seg_of_row(p.cu_seqlens, p.n_segs, row, lane);
+  auto ld = [](const auto* q) { return io<std::decay_t<decltype(*q)>>::ld(q); };
+  auto stats = [&](auto&& value, float* r0, float* r1, float& mean, float& inv) {
+    mean = 0.f;
+    if (p.kind == SJ_NORM_LN) {
+      float s = 0.f;
+      for (int k = threadIdx.x; k < p.D; k += blockDim.x) s += value(k);
+      mean = group_sum<false>(s, r0) * inv_d;
+    }
+    float q = 0.f;
+    for (int k = threadIdx.x; k < p.D; k += blockDim.x) {
+      const float d = value(k) - mean;
+      q += d * d;
+    }
+    inv = rsqrtf(group_sum<false>(q, r1) * inv_d + p.eps);
+  };
+  float zm = 0.f, zi = 1.f, xm, xi;
+  if (p.post_w) stats([&](int k) { return ld(r + k); }, red[0], red[1], zm, zi);
+  auto stream = [&](int k) {
+    float z = ld(r + k);
+    if (p.post_w) {
+      z = (z - zm) * zi * p.post_w[k];
+      if (p.post_b) z += p.post_b[k];
+    }
+    if (p.gate_mode == SJ_GATE_ROW)
+      z *= sigmoid(p.gate_type == SJ_TYPE_BF16
+                       ? __bfloat162float(static_cast<const bf16*>(p.gate)[row * p.ldg + k])
+                       : static_cast<const float*>(p.gate)[row * p.ldg + k]);
+    else if (p.gate_mode != SJ_GATE_NONE)
+      z *= static_cast<const float*>(p.gate)[(int64_t)seg * p.D + k];
+    return p.alpha * ld(x + k) + p.beta * z;
+  };
+  if (p.y) stats(stream, red[2], red[3], xm, xi);
+  TX* xo = static_cast<TX*>(p.x_out) + row * p.ldxo;
+  TY* y = static_cast<TY*>(p.y) + row * p.ldy;
+  for (int k = threadIdx.x; k < p.D; k += blockDim.x) {
+    const float v = stream(k);
+    xo[k] = io<TX>::cvt(v);
+    if (p.y) {
+      float o = (v - xm) * xi * p.pre_w[k];
+      if (p.pre_b) o += p.pre_b[k];
+      y[k] = io<TY>::cvt(o);
+    }
+  }
+}
+
+template <typename TX, typename TR, typename TY, int VEC, bool WARP>
+cudaError_t launch(const sj_norm_block_args& a, int group, cudaStream_t st) {
+  const int nc = ((a.D + VEC - 1) / VEC + group - 1) / group;
+  const int rows_per_block = WARP ? 4 : 1;
+  const int threads = WARP ? 128 : group;
+  const int64_t blocks = (a.M + rows_per_block - 1) / rows_per_block;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  auto go = [&](auto kernel) {
+    kernel<<<(unsigned)blocks, threads, 0, st>>>(a);
+    return cudaGetLastError();
+  };
+  if (nc <= 2) return go(norm_block_kernel<TX, TR, TY, VEC, 2, WARP>);
+  if (nc <= 4) return go(norm_block_kernel<TX, TR, TY, VEC, 4, WARP>);
+  if constexpr (WARP || VEC == 1) {  // blocks take at most 4 chunks of 4 (dispatch)
+    if (nc <= 6) return go(norm_block_kernel<TX, TR, TY, VEC, 6, WARP>);
+    if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, VEC, 8, WARP>);
+  }
+  return cudaErrorInvalidConfiguration;
+}
+
+template <typename TX, typename TR, typename TY>
+cudaError_t dispatch(const sj_norm_block_args& a, cudaStream_t st) {
+  // whole vectors of 4: the width, every pitch and every address
+  auto on = [](const void* p, int type) {
+    return !(reinterpret_cast<uintptr_t>(p) & (type == SJ_TYPE_BF16 ? 7 : 15));
+  };
+  const bool row_gate = a.gate_mode == SJ_GATE_ROW;
+  const bool vec4 = a.D % 4 == 0 && a.ldx % 4 == 0 && a.ldxo % 4 == 0 && a.ldr % 4 == 0 &&
+                    (!a.y || a.ldy % 4 == 0) && (!row_gate || a.ldg % 4 == 0) &&
+                    on(a.x, a.x_type) && on(a.x_out, a.x_type) && on(a.r, a.r_type) &&
+                    on(a.y, a.y_type) && on(a.post_w, 0) && on(a.post_b, 0) && on(a.pre_w, 0) &&
+                    on(a.pre_b, 0) && on(a.gate, row_gate ? a.gate_type : 0);
+  const int chunks = vec4 ? a.D / 4 : a.D;
+  if (chunks <= 32 * 8) {
+    return vec4 ? launch<TX, TR, TY, 4, true>(a, 32, st) : launch<TX, TR, TY, 1, true>(a, 32, st);
+  }
+  int group = 64;
+  while (group < 1024 && chunks > 4 * group) group *= 2;
+  if (chunks <= 4 * group || (!vec4 && chunks <= 8 * group))
+    return vec4 ? launch<TX, TR, TY, 4, false>(a, group, st)
+                : launch<TX, TR, TY, 1, false>(a, group, st);
+  if (a.M > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  norm_block_wide<TX, TR, TY><<<(unsigned)a.M, 1024, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename TX, typename TR>
+cudaError_t dispatch_y(const sj_norm_block_args& a, cudaStream_t st) {
+  return a.y_type == SJ_TYPE_BF16 ? dispatch<TX, TR, bf16>(a, st) : dispatch<TX, TR, float>(a, st);
+}
+
+}  // namespace
+
+cudaError_t norm_block(const sj_norm_block_args& a, cudaStream_t st) {
+  if (a.x_type == SJ_TYPE_BF16)
+    return a.r_type == SJ_TYPE_BF16 ? dispatch_y<bf16, bf16>(a, st) : dispatch_y<bf16, float>(a, st);
+  return a.r_type == SJ_TYPE_BF16 ? dispatch_y<float, bf16>(a, st) : dispatch_y<float, float>(a, st);
+}
+
+}  // namespace sjb
+
+namespace {
+int bad(const char* m) {
+  sjb::set_last_error(m);
+  return SJ_ERR_INVALID;
+}
+}  // namespace
+
+extern "C" int sj_norm_block(const sj_norm_block_args* a, void* stream) {
+  if (!a) return bad("null norm argument");
+  auto type = [](int t) { return t == SJ_TYPE_F32 || t == SJ_TYPE_BF16; };
+  if (a->M < 0 || a->D <= 0) return bad("bad norm size");
+  if (!type(a->x_type) || !type(a->r_type) || (a->y && !type(a->y_type)))
+    return bad("types must be SJ_TYPE_F32 or SJ_TYPE_BF16");
+  if (a->kind != SJ_NORM_LN && a->kind != SJ_NORM_RMS)
+    return bad("kind must be SJ_NORM_LN or SJ_NORM_RMS");
+  if (!(a->eps >= 0.f)) return bad("eps must not be negative");
+  if (a->gate_mode < SJ_GATE_NONE || a->gate_mode > SJ_GATE_ROW) return bad("bad gate_mode");
+  if (a->M == 0) return SJ_OK;
+  if (!a->x || !a->x_out || !a->r) return bad("null norm operand");
+  if (a->y && !a->pre_w) return bad("y needs pre_w");
+  if ((a->post_b && !a->post_w) || (a->pre_b && !a->pre_w)) return bad("a bias needs its weight");
+  if (a->ldx < a->D || a->ldxo < a->D || a->ldr < a->D || (a->y && a->ldy < a->D))
+    return bad("a row pitch is smaller than its row");
+  if (a->gate_mode != SJ_GATE_NONE && !a->gate) return bad("gate is null");
+  if (a->gate_mode == SJ_GATE_SEGMENT && (!a->cu_seqlens || a->n_segs <= 0))
+    return bad("a gate for each segment needs cu_seqlens");
+  if (a->gate_mode == SJ_GATE_ROW && (a->ldg < a->D || !type(a->gate_type)))
+    return bad("bad gate pitch or type");
+  const cudaError_t rc = sjb::norm_block(*a, static_cast<cudaStream_t>(stream));
+  if (rc == cudaSuccess) return SJ_OK;
+  sjb::set_last_error(std::string("snapjudge CUDA: norm_block: ") + cudaGetErrorString(rc));
+  return SJ_ERR_CUDA;
+}

@@ -5,6 +5,12 @@ Thin wrappers over the C ABI launchers (``sj_gemm``, ``sj_gemm_geglu``,
 ``cuda/kernels.cu`` entry points.  Tensors must be contiguous CUDA tensors of
 the documented dtypes; the launch is asynchronous on torch's current stream.
 torch is used only to own device memory and streams.
+
+The operators of an encoder layer (``attn_masked``, ``gemm_lora``,
+``norm_block``) have no counterpart in the reference.  Two of them take a plan,
+made once per batch from its lengths (``AttnPlan``, ``LoraPlan``) and used in
+every layer; a plan is complete on the device when its constructor returns and
+may be used on any stream.
 """
 from __future__ import annotations
 
@@ -117,3 +123,224 @@ def gemm_e4m3(A, sa, W, sw, bias=None, act=0, geglu=False):
     check(_lib.lib().sj_gemm_e4m3(_p(A), _p(W), _p(sa), _p(sw), _p(bias), _p(C_), M, N, K,
                                   int(bias is not None), act, int(geglu), _stream()))
     return C_
+
+
+def _host_i32(a, name):
+    """A host array of whole numbers as contiguous int32 (refused if a value does not fit)."""
+    if a is None:
+        return None
+    a = np.asarray(a)
+    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+        raise ValueError(f"{name} must be a 1-D array of whole numbers")
+    b = np.ascontiguousarray(a, np.int32)
+    if a.size and not np.array_equal(a, b):
+        raise ValueError(f"{name} has values that do not fit in 32 bits")
+    return b
+
+
+def _plan_on_device(buf, device):
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    t = torch.from_numpy(buf).to(dev)
+    torch.cuda.current_stream(t.device).synchronize()
+    return t
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t, name, dtype):
+    """A CUDA tensor whose last dimension is contiguous; returns its row pitch in elements."""
+    if not (t.is_cuda and t.dtype == dtype and t.dim() == 2):
+        raise ValueError(f"{name} must be a 2-D CUDA {dtype} tensor")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vec(t, name, n):
+    """A contiguous CUDA fp32 tensor of shape n (or None)."""
+    if t is not None:
+        _need(t, torch.float32, name)
+        if tuple(t.shape) != n:
+            raise ValueError(f"{name} must have shape {n}, not {tuple(t.shape)}")
+
+
+class AttnPlan:
+    """Which keys each query row of a packed batch sees, for :func:`attn_masked`.
+
+    ``cu`` (host, [B + 1]) are the cumulative lengths of the segments.  Query row
+    ``i`` sees key row ``j`` of its segment (``jr`` = j's place in it) iff
+    ``jr < kv_lens[b]`` and (``jr < prefix[b]`` or (j is in i's document, and
+    ``j <= i`` when ``causal``, and ``|i - j| <= window`` when ``window > 0``)).
+    ``docs``: host row boundaries of the documents, a refinement of ``cu``
+    (None: a segment is one document); ``prefix``, ``kv_lens``: host [B] or None;
+    ``q_rows``: strictly increasing packed rows that ask (None: all).
+    """
+
+    def __init__(self, cu, *, docs=None, prefix=None, kv_lens=None, q_rows=None, causal=False,
+                 window=0, device=None):
+        cu = _host_i32(cu, "cu")
+        docs, prefix = _host_i32(docs, "docs"), _host_i32(prefix, "prefix")
+        kv_lens, q_rows = _host_i32(kv_lens, "kv_lens"), _host_i32(q_rows, "q_rows")
+        if cu is None or not len(cu):
+            raise ValueError("cu must have at least one value")
+        B = len(cu) - 1
+        for a, name in ((prefix, "prefix"), (kv_lens, "kv_lens")):
+            if a is not None and len(a) != B:
+                raise ValueError(f"{name} must have one value for each segment")
+        if docs is not None and not len(docs):
+            raise ValueError("docs must have at least one value")
+        p = lambda a: None if a is None else a.ctypes.data  # noqa: E731
+        args = _lib.AttnPlanArgs(p(cu), B, p(docs), 0 if docs is None else len(docs) - 1, p(prefix),
+                                 p(kv_lens), p(q_rows), 0 if q_rows is None else len(q_rows),
+                                 int(causal), int(window))
+        self.info = _lib.AttnPlanInfo()
+        L = _lib.lib()
+        check(L.sj_attn_plan(C.byref(args), None, 0, C.byref(self.info)))
+        buf = np.empty(max(1, self.info.plan_len), np.int32)
+        check(L.sj_attn_plan(C.byref(args), buf.ctypes.data, len(buf), C.byref(self.info)))
+        self.n_rows, self.n_keys = self.info.n_rows, self.info.n_keys
+        self.data = _plan_on_device(buf, device)
+
+
+def _heads(t, name):
+    """[rows, heads, Dh] bf16 with contiguous rows of heads; returns its row pitch."""
+    if not (t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 3):
+        raise ValueError(f"{name} must be a [rows, heads, head_dim] CUDA bfloat16 tensor")
+    n, H, Dh = t.shape
+    if (Dh > 1 and t.stride(2) != 1) or (H > 1 and t.stride(1) != Dh):
+        raise ValueError(f"{name}: a row's heads must be contiguous")
+    return t.stride(0) if n > 1 else H * Dh
+
+
+def attn_masked(q, k, v, plan, *, scale=None, softcap=0.0, rel_bias=None, slopes=None):
+    """Attention over the keys that ``plan`` shows each row -> bf16 [rows, H * Dh].
+
+    q [plan.n_rows, H, Dh], k and v [plan.n_keys, Hkv, Dh] bf16 (slices of a
+    packed tensor are fine), H a multiple of Hkv.  The score of a pair at
+    distance d = j - i is ``scale q.k`` (scale None: 1 / sqrt(Dh)), capped to
+    ``softcap tanh(x / softcap)`` when softcap > 0, plus ``rel_bias[h,
+    clamp(d, -R, R) + R]`` (fp32 [H, 2R + 1]), minus ``slopes[h] |d|`` (fp32
+    [H]).  A row that sees no key gives 0."""
+    ldq, ldk, ldv = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    n, H, Dh = q.shape
+    Hkv = k.shape[1]
+    if n != plan.n_rows or k.shape[0] != plan.n_keys or v.shape != k.shape or k.shape[2] != Dh:
+        raise ValueError("q must have plan.n_rows rows, k and v plan.n_keys, of one head_dim")
+    if H == 0 or Hkv == 0 or H % Hkv:
+        raise ValueError("q's heads must be a multiple of k's")
+    R = 0
+    if rel_bias is not None:
+        if rel_bias.dim() != 2 or rel_bias.shape[1] % 2 == 0:
+            raise ValueError("rel_bias must be [H, 2R + 1]")
+        R = rel_bias.shape[1] // 2
+        _vec(rel_bias, "rel_bias", (H, 2 * R + 1))
+    _vec(slopes, "slopes", (H,))
+    L = _lib.lib()
+    O = torch.empty(n, H * Dh, dtype=torch.bfloat16, device=q.device)
+    need = L.sj_attn_masked_workspace(C.byref(plan.info), H, Hkv, Dh)
+    if need < 0:
+        check(_lib.SJ_ERR_INVALID)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    args = _lib.AttnMaskedArgs(_at(q), _at(k), _at(v), _at(O), ldq, ldk, ldv, H * Dh, H, Hkv, Dh,
+                               Dh ** -0.5 if scale is None else scale, softcap, _at(rel_bias), R,
+                               _at(slopes))
+    check(L.sj_attn_masked(C.byref(args), C.byref(plan.info), _at(plan.data), _at(ws), need,
+                           _stream()))
+    return O
+
+
+class LoraPlan:
+    """Which adapter each row of a packed batch uses, for :func:`gemm_lora`:
+    segment b of ``cu`` (host cumulative lengths) uses adapter ``ids[b]`` of
+    ``n_adapters``, or none (-1); ``rank`` is the adapters' rank."""
+
+    def __init__(self, cu, ids, *, rank, n_adapters, device=None):
+        cu, ids = _host_i32(cu, "cu"), _host_i32(ids, "ids")
+        if cu is None or ids is None or len(cu) != len(ids) + 1:
+            raise ValueError("cu must have one value more than ids")
+        self.info = _lib.LoraPlanInfo()
+        L = _lib.lib()
+        a = (cu.ctypes.data, len(ids), ids.ctypes.data, n_adapters, rank)
+        check(L.sj_lora_plan(*a, None, 0, C.byref(self.info)))
+        buf = np.empty(max(1, self.info.plan_len), np.int32)
+        check(L.sj_lora_plan(*a, buf.ctypes.data, len(buf), C.byref(self.info)))
+        self.n_rows, self.rank, self.n_adapters = self.info.M, rank, n_adapters
+        self.data = _plan_on_device(buf, device)
+
+
+def gemm_lora(X, W, A, B, plan, *, scale=None, bias=None, act=0):
+    """bf16 act(X W^T + bias + scale[a] (X A[a]^T) B[a]^T), a = the row's adapter
+    in ``plan`` (rows without one: no such term).  X [M, K], W [N, K], A
+    [n_adapters, rank, K], B [n_adapters, N, rank] bf16; scale [n_adapters] and
+    bias [N] fp32; act as in :func:`gemm`."""
+    ldx = _rows(X, "X", torch.bfloat16)
+    for t, name in ((W, "W"), (A, "A"), (B, "B")):
+        _need(t, torch.bfloat16, name)
+    M, K = X.shape
+    N = W.shape[0]
+    if M != plan.n_rows or tuple(W.shape) != (N, K):
+        raise ValueError("X must have plan.n_rows rows, and W the columns of X")
+    if tuple(A.shape) != (plan.n_adapters, plan.rank, K):
+        raise ValueError("A must be [n_adapters, rank, K]")
+    if tuple(B.shape) != (plan.n_adapters, N, plan.rank):
+        raise ValueError("B must be [n_adapters, N, rank]")
+    _vec(scale, "scale", (plan.n_adapters,))
+    _vec(bias, "bias", (N,))
+    L = _lib.lib()
+    C_ = torch.empty(M, N, dtype=torch.bfloat16, device=X.device)
+    need = L.sj_gemm_lora_workspace(C.byref(plan.info), N, K)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=X.device)
+    args = _lib.GemmLoraArgs(_at(X), _at(W), _at(A), _at(B), _at(scale), _at(bias), _at(C_), ldx, N,
+                             N, K, act)
+    check(L.sj_gemm_lora(C.byref(args), C.byref(plan.info), _at(plan.data), _at(ws), need,
+                         _stream()))
+    return C_
+
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_KINDS = {"ln": 0, "rms": 1}
+
+
+def norm_block(X, R, pre_w=None, pre_b=None, *, post_w=None, post_b=None, kind="ln", eps=1e-5,
+               gate=None, cu=None, alpha=1.0, beta=1.0, out_dtype=torch.bfloat16, inplace=False):
+    """The step between two blocks: z = post_norm(R) (R itself without post_w),
+    X' = alpha X + beta g z, Y = pre_norm(X') -> (X', Y), Y None without pre_w.
+
+    X, R [M, D] fp32 or bf16; weights and biases fp32 [D]; kind "ln" or "rms".
+    gate: fp32 [D]; or, with cu (device int32 cumulative lengths), fp32
+    [len(cu) - 1, D], a row for each segment; or [M, D] fp32 or bf16, through a
+    sigmoid.  X' has X's type and is X itself with inplace; Y has out_dtype."""
+    if X.dtype not in _TYPES or R.dtype not in _TYPES or out_dtype not in _TYPES:
+        raise ValueError("X, R and Y must be float32 or bfloat16")
+    if kind not in _KINDS:
+        raise ValueError("kind must be 'ln' or 'rms'")
+    ldx, ldr = _rows(X, "X", X.dtype), _rows(R, "R", R.dtype)
+    M, D = X.shape
+    if R.shape != X.shape:
+        raise ValueError("R must have X's shape")
+    for t, name in ((post_w, "post_w"), (post_b, "post_b"), (pre_w, "pre_w"), (pre_b, "pre_b")):
+        _vec(t, name, (D,))
+    mode = gtype = ldg = n_segs = 0
+    if gate is not None:
+        if cu is not None:
+            mode, n_segs = 2, cu.numel() - 1
+            _need(cu, torch.int32, "cu")
+            _vec(gate, "gate", (n_segs, D))
+        elif gate.dim() == 1:
+            mode = 1
+            _vec(gate, "gate", (D,))
+        else:
+            mode = 3
+            if gate.dtype not in _TYPES or gate.shape != X.shape:
+                raise ValueError("gate must be [D], [segments, D] with cu, or [M, D]")
+            gtype, ldg = _TYPES[gate.dtype], _rows(gate, "gate", gate.dtype)
+    Xo = X if inplace else torch.empty(M, D, dtype=X.dtype, device=X.device)
+    Y = None if pre_w is None else torch.empty(M, D, dtype=out_dtype, device=X.device)
+    args = _lib.NormBlockArgs(_at(X), _at(Xo), _at(R), _at(Y), _TYPES[X.dtype], _TYPES[R.dtype],
+                              _TYPES[out_dtype], ldx, ldx if inplace else D, ldr, D, _at(post_w),
+                              _at(post_b), _at(pre_w), _at(pre_b), _KINDS[kind], eps, _at(gate),
+                              mode, gtype, ldg, _at(cu), n_segs, alpha, beta, M, D)
+    check(_lib.lib().sj_norm_block(C.byref(args), _stream()))
+    return Xo, Y

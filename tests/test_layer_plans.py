@@ -1,0 +1,275 @@
+"""Plans of the encoder-layer operators, built on the host: which keys each query
+row sees (sj_attn_plan) and which adapters each block of rows needs
+(sj_lora_plan), against their definitions; and the refusals of all three
+operators.  No GPU."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from snapjudge_b200 import _lib
+
+
+def _p(a):
+    return None if a is None else a.ctypes.data
+
+
+def _i32(a):
+    return None if a is None else np.ascontiguousarray(a, np.int32)
+
+
+def attn_plan(cu, docs=None, prefix=None, kv_lens=None, q_rows=None, causal=0, window=0):
+    cu, docs, prefix, kv_lens, q_rows = map(_i32, (cu, docs, prefix, kv_lens, q_rows))
+    a = _lib.AttnPlanArgs(_p(cu), len(cu) - 1, _p(docs), 0 if docs is None else len(docs) - 1,
+                          _p(prefix), _p(kv_lens), _p(q_rows), 0 if q_rows is None else len(q_rows),
+                          causal, window)
+    info = _lib.AttnPlanInfo()
+    L = _lib.lib()
+    rc = L.sj_attn_plan(C.byref(a), None, 0, C.byref(info))
+    if rc:
+        return rc, None, None
+    buf = np.full(info.plan_len + 1, 77, np.int32)
+    assert L.sj_attn_plan(C.byref(a), buf.ctypes.data, info.plan_len, C.byref(info)) == 0
+    assert buf[-1] == 77  # nothing written past the plan
+    if info.plan_len:
+        assert L.sj_attn_plan(C.byref(a), buf.ctypes.data, info.plan_len - 1,
+                              C.byref(info)) == _lib.SJ_ERR_INVALID
+    return 0, info, buf[:-1]
+
+
+def visible(cu, docs=None, prefix=None, kv_lens=None, q_rows=None, causal=0, window=0):
+    """bool [query rows, keys] from the definition, pair by pair."""
+    T = cu[-1]
+    seg = np.repeat(np.arange(len(cu) - 1), np.diff(cu))
+    doc = seg if docs is None else np.repeat(np.arange(len(docs) - 1), np.diff(docs))
+    rows = range(T) if q_rows is None else q_rows
+    out = np.zeros((len(rows), T), bool)
+    for r, i in enumerate(rows):
+        for j in range(T):
+            b = seg[i]
+            if seg[j] != b:
+                continue
+            jr = j - cu[b]
+            if kv_lens is not None and jr >= kv_lens[b]:
+                continue
+            pre = prefix is not None and jr < prefix[b]
+            out[r, j] = pre or (doc[i] == doc[j] and (not causal or j <= i)
+                                and (window == 0 or abs(i - j) <= window))
+    return out
+
+
+CASES = [
+    dict(cu=[0, 1]),
+    dict(cu=[0, 0, 5, 5, 9, 9]),  # empty segments
+    dict(cu=[0, 300, 301, 450]),
+    dict(cu=[0, 300, 301, 450], window=40),
+    dict(cu=[0, 300, 301, 450], window=2**31 - 1),
+    dict(cu=[0, 300, 301, 450], causal=1),
+    dict(cu=[0, 300, 301, 450], causal=1, prefix=[100, 0, 149], kv_lens=[290, 0, 2**31 - 1]),
+    dict(cu=[0, 200, 330], docs=[0, 120, 150, 200, 260, 330], prefix=[120, 60]),
+    dict(cu=[0, 200, 330], docs=[0, 120, 120, 150, 200, 200, 260, 330], prefix=[50, 130], window=7,
+         kv_lens=[180, 100]),
+    dict(cu=[0, 200, 330], docs=[0, 5, 150, 200, 260, 330], causal=1, window=33),
+    dict(cu=[0, 400, 700, 900], q_rows=[0, 17, 399, 400, 899], prefix=[3, 0, 200]),
+    dict(cu=[0, 400, 700], q_rows=[]),
+    dict(cu=[0, 64, 128, 192, 256]),
+    dict(cu=np.concatenate([[0], np.cumsum(np.random.default_rng(4).integers(0, 30, 40))])),
+]
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_attn_plan_shows_the_defined_keys(case):
+    want = visible(**case)
+    rc, info, plan = attn_plan(**case)
+    assert rc == 0 and info.n_rows == want.shape[0] and info.n_keys == want.shape[1]
+    rows = plan[:8 * info.n_rows].reshape(-1, 8)
+    got = np.zeros_like(want)
+    for r, (pos, a0, a1, b0, b1) in enumerate(rows[:, :5]):
+        assert pos == (r if case.get("q_rows") is None else case["q_rows"][r])
+        assert a0 <= a1 <= b0 <= b1 and (a1 > a0 or b1 == b0)
+        got[r, a0:a1] = True
+        got[r, b0:b1] = True
+    assert (got == want).all()
+    # items: every query row in one; their key tiles cover what the rows see, once
+    items = plan[info.off_items:info.off_tiles].reshape(-1, 4)
+    tiles = plan[info.off_tiles:]
+    seen = np.zeros(info.n_rows, int)
+    assert (np.diff(items[:, 3]) <= 0).all()  # longest first
+    for row0, n, t0, nt in items:
+        assert 1 <= n <= 128
+        seen[row0:row0 + n] += 1
+        cover = np.zeros(want.shape[1] + 64, int)
+        for t in tiles[t0:t0 + nt]:
+            k0 = ~t if t < 0 else t
+            cover[k0:k0 + 64] += 1
+            sub = want[row0:row0 + n, k0:k0 + 64]
+            assert sub.any()
+            assert (t < 0) == (sub.shape[1] == 64 and sub.all())
+        assert cover.max(initial=0) <= 1
+        assert (cover[:want.shape[1]][want[row0:row0 + n].any(0)] == 1).all()
+    assert (seen == 1).all()
+
+
+@pytest.mark.parametrize("case,word", [
+    (dict(cu=[1, 5]), b"cu_seqlens[0]"),
+    (dict(cu=[0, 5, 3]), b"non-decreasing"),
+    (dict(cu=[0, 5], window=-1), b"window"),
+    (dict(cu=[0, 5], prefix=[6]), b"prefix"),
+    (dict(cu=[0, 5], prefix=[-1]), b"prefix"),
+    (dict(cu=[0, 5], kv_lens=[-1]), b"kv_lens"),
+    (dict(cu=[0, 5, 9], docs=[0, 4, 9]), b"boundary"),
+    (dict(cu=[0, 5], docs=[0, 4]), b"end at the last row"),
+    (dict(cu=[0, 5], docs=[0, 4, 2, 5]), b"non-decreasing"),
+    (dict(cu=[0, 5], q_rows=[1, 1]), b"increasing"),
+    (dict(cu=[0, 5], q_rows=[5]), b"increasing"),
+    (dict(cu=[0, 5], q_rows=[-1]), b"increasing"),
+])
+def test_attn_plan_refuses(case, word):
+    rc, _, _ = attn_plan(**case)
+    assert rc == _lib.SJ_ERR_INVALID and word in _lib.lib().sj_last_error()
+
+
+def lora_plan(cu, ids, n, rank):
+    cu, ids = _i32(cu), _i32(ids)
+    info = _lib.LoraPlanInfo()
+    L = _lib.lib()
+    rc = L.sj_lora_plan(_p(cu), len(ids), _p(ids), n, rank, None, 0, C.byref(info))
+    if rc:
+        return rc, None, None
+    buf = np.full(info.plan_len + 1, 77, np.int32)
+    assert L.sj_lora_plan(_p(cu), len(ids), _p(ids), n, rank, buf.ctypes.data, info.plan_len,
+                          C.byref(info)) == 0
+    assert buf[-1] == 77
+    return 0, info, buf[:-1]
+
+
+@pytest.mark.parametrize("cu,ids,n,rank", [
+    ([0], [], 0, 1),
+    ([0, 1], [-1], 3, 16),
+    ([0, 1], [2], 3, 8),
+    ([0, 0, 255, 256, 257, 257, 1000], [1, 0, 2, 0, 1, 2], 3, 24),
+    ([0, 0, 0, 700, 700, 701], [0, 1, 2, 0, -1], 3, 64),
+    (np.arange(601), np.random.default_rng(3).integers(-1, 64, 600), 64, 16),
+])
+def test_lora_plan_lists_each_blocks_adapters(cu, ids, n, rank):
+    rc, info, plan = lora_plan(cu, ids, n, rank)
+    assert rc == 0
+    rows = np.repeat(np.asarray(ids, int), np.diff(cu))
+    assert info.M == len(rows) and (plan[:info.M] == rows).all()
+    first = plan[info.off_blocks:info.off_blocks + info.n_blocks + 1]
+    slabs = plan[info.off_slabs:info.off_slabs + 2 * info.n_slabs].reshape(-1, 2)
+    assert info.n_blocks == -(-info.M // 256) and first[0] == 0 and first[-1] == info.n_slabs
+    for k in range(info.n_blocks):
+        want = {(a, s) for a in set(rows[256 * k:256 * k + 256].tolist()) - {-1}
+                for s in range(-(-rank // 16))}
+        mine = [tuple(x) for x in slabs[first[k]:first[k + 1]].tolist()]
+        assert len(mine) == len(want) and set(mine) == want
+
+
+@pytest.mark.parametrize("cu,ids,n,rank,word", [
+    ([1, 5], [0], 1, 8, b"cu_seqlens[0]"),
+    ([0, 5, 3], [0, 0], 1, 8, b"non-decreasing"),
+    ([0, 5], [1], 1, 8, b"adapter number"),
+    ([0, 5], [-2], 1, 8, b"adapter number"),
+    ([0, 5], [0], 1, 0, b"rank"),
+    ([0, 5], [0], -1, 8, b"negative"),
+])
+def test_lora_plan_refuses(cu, ids, n, rank, word):
+    rc, _, _ = lora_plan(cu, ids, n, rank)
+    assert rc == _lib.SJ_ERR_INVALID and word in _lib.lib().sj_last_error()
+
+
+def _bad(rc, word):
+    assert rc == _lib.SJ_ERR_INVALID and word in _lib.lib().sj_last_error(), \
+        (rc, _lib.lib().sj_last_error())
+
+
+def test_attn_masked_refuses_on_the_host():
+    L = _lib.lib()
+    _, info, _ = attn_plan([0, 5])
+    one = 16  # never read: every call below is refused before a launch
+
+    def call(plan=one, ws=None, wsb=0, **kw):
+        d = dict(q=one, k=one, v=one, O=one, ldq=128, ldk=128, ldv=128, ldo=128, H=2, Hkv=1, Dh=64,
+                 scale=0.1, softcap=0.0, rel_bias=None, rel_max=0, slopes=None)
+        d.update(kw)
+        a = _lib.AttnMaskedArgs(*[d[f] for f, _ in _lib.AttnMaskedArgs._fields_])
+        return L.sj_attn_masked(C.byref(a), C.byref(info), plan, ws, wsb, None)
+
+    _bad(call(H=3, Hkv=2), b"multiple")
+    _bad(call(H=0), b"multiple")
+    _bad(call(Hkv=0), b"multiple")
+    _bad(call(Dh=129, ldq=512, ldk=512, ldv=512, ldo=512), b"head_dim")
+    _bad(call(Dh=0), b"head_dim")
+    _bad(call(softcap=-1.0), b"softcap")
+    _bad(call(softcap=float("inf")), b"softcap")
+    _bad(call(softcap=float("nan")), b"softcap")
+    _bad(call(scale=float("nan")), b"scale")
+    _bad(call(rel_bias=one, rel_max=-1), b"rel_max")
+    _bad(call(ldq=127), b"pitch")
+    _bad(call(ldk=63), b"pitch")
+    _bad(call(ldo=100), b"pitch")
+    for f in ("q", "k", "v", "O"):
+        _bad(call(**{f: None}), b"null")
+    _bad(call(plan=None), b"null")
+    assert L.sj_attn_masked(None, C.byref(info), None, None, 0, None) == _lib.SJ_ERR_INVALID
+    assert L.sj_attn_masked_workspace(C.byref(info), 3, 2, 64) == -1
+    _, empty, _ = attn_plan([0, 0])
+    a = _lib.AttnMaskedArgs(H=1, Hkv=1, Dh=64, scale=1.0)
+    assert L.sj_attn_masked(C.byref(a), C.byref(empty), None, None, 0, None) == 0  # nothing to do
+
+
+def test_gemm_lora_refuses_on_the_host():
+    L = _lib.lib()
+    _, info, _ = lora_plan([0, 5], [0], 1, 8)
+    one = 16
+
+    def call(plan=one, ws=one, wsb=1 << 20, **kw):
+        d = dict(X=one, W=one, A=one, Bw=one, scale=None, bias=None, C=one, ldx=64, ldc=32, N=32,
+                 K=64, act=0)
+        d.update(kw)
+        a = _lib.GemmLoraArgs(*[d[f] for f, _ in _lib.GemmLoraArgs._fields_])
+        return L.sj_gemm_lora(C.byref(a), C.byref(info), plan, ws, wsb, None)
+
+    _bad(call(N=-1), b"negative")
+    _bad(call(act=3), b"act")
+    _bad(call(ldx=63), b"pitch")
+    _bad(call(ldc=31), b"pitch")
+    for f in ("X", "W", "A", "Bw", "C"):
+        _bad(call(**{f: None}), b"null")
+    _bad(call(plan=None), b"null")
+    _bad(call(wsb=0), b"workspace")
+    _bad(call(ws=None), b"workspace")
+    assert L.sj_gemm_lora_workspace(C.byref(info), -1, 4) == -1
+
+
+def test_norm_block_refuses_on_the_host():
+    L = _lib.lib()
+    one = 16
+
+    def call(**kw):
+        d = dict(x=one, x_out=one, r=one, y=one, x_type=0, r_type=1, y_type=1, ldx=8, ldxo=8, ldr=8,
+                 ldy=8, post_w=None, post_b=None, pre_w=one, pre_b=None, kind=0, eps=1e-5,
+                 gate=None, gate_mode=0, gate_type=0, ldg=0, cu_seqlens=None, n_segs=0, alpha=1.0,
+                 beta=1.0, M=1, D=8)
+        d.update(kw)
+        a = _lib.NormBlockArgs(*[d[f] for f, _ in _lib.NormBlockArgs._fields_])
+        return L.sj_norm_block(C.byref(a), None)
+
+    _bad(call(M=-1), b"size")
+    _bad(call(D=0), b"size")
+    _bad(call(x_type=2), b"types")
+    _bad(call(y_type=7), b"types")
+    _bad(call(kind=2), b"kind")
+    _bad(call(eps=-1.0), b"eps")
+    _bad(call(eps=float("nan")), b"eps")
+    _bad(call(gate_mode=4), b"gate_mode")
+    _bad(call(x=None), b"null")
+    _bad(call(r=None), b"null")
+    _bad(call(pre_w=None), b"pre_w")
+    _bad(call(post_b=one), b"weight")
+    _bad(call(ldr=7), b"pitch")
+    _bad(call(gate_mode=1), b"gate")
+    _bad(call(gate_mode=2, gate=one), b"cu_seqlens")
+    _bad(call(gate_mode=3, gate=one, ldg=7), b"gate pitch")
+    assert call(M=0) == 0
