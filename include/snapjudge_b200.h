@@ -118,7 +118,8 @@ int sj_attn_noalloc(const sj_bf16* qkv, const int32_t* cu_seqlens, const int32_t
  * out (the kernel stops issuing, waits for its own copies, frees its
  * resources and returns early, leaving its output incomplete) is recorded in
  * a status word of the library, one per device, shared by every call of
- * sj_gemm, sj_gemm_geglu, sj_attn, sj_attn_noalloc and sj_gemm_e4m3.  This
+ * sj_gemm, sj_gemm_geglu, sj_attn, sj_attn_noalloc, sj_gemm_e4m3,
+ * sj_attn_masked and sj_gemm_lora.  This
  * call waits for `stream`, returns SJ_ERR_TIMEOUT (message in sj_last_error)
  * if any of those calls recorded one since the last check, and clears the
  * word.  Call it where the reference would check cudaGetLastError after a
@@ -240,6 +241,7 @@ typedef struct sj_lora_plan_info {
   int32_t rank, n_adapters;
   int32_t n_blocks;  /* blocks of 256 rows */
   int32_t n_slabs;   /* (block, adapter, 16 of its ranks) */
+  int32_t max_slabs; /* of one block */
   int64_t off_blocks, off_slabs; /* word offsets into the plan */
 } sj_lora_plan_info;
 

@@ -84,7 +84,7 @@ class AttnMaskedArgs(C.Structure):
 class LoraPlanInfo(C.Structure):
     _fields_ = [("plan_len", _L), ("M", C.c_int32), ("rank", C.c_int32),
                 ("n_adapters", C.c_int32), ("n_blocks", C.c_int32), ("n_slabs", C.c_int32),
-                ("off_blocks", _L), ("off_slabs", _L)]
+                ("max_slabs", C.c_int32), ("off_blocks", _L), ("off_slabs", _L)]
 
 
 class GemmLoraArgs(C.Structure):

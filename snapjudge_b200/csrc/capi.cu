@@ -11,6 +11,7 @@
 
 #include "../../include/snapjudge_b200.h"
 #include "common.cuh"
+#include "gemm_lora.cuh"
 #include "kernels.h"
 
 using sjb::bf16;
@@ -180,12 +181,14 @@ int sj_check_device_errors(void* stream) {
   auto st = static_cast<cudaStream_t>(stream);
   cudaError_t rc = cudaStreamSynchronize(st);
   if (rc != cudaSuccess) return launched(rc, "cudaStreamSynchronize");
-  int a = 0, g = 0, sc = 0, al = 0;
+  int a = 0, g = 0, sc = 0, al = 0, gl = 0;
   if ((rc = sjb::attn_tc_take_status(&a)) != cudaSuccess) return launched(rc, "attention status");
   if ((rc = sjb::attn_long_take_status(&al)) != cudaSuccess)
     return launched(rc, "attention status");
   if (!a) a = al;
   if ((rc = sjb::gemm_tc_take_status(&g)) != cudaSuccess) return launched(rc, "GEMM status");
+  if ((rc = sjb::gemm_lora_take_status(&gl)) != cudaSuccess) return launched(rc, "GEMM status");
+  if (!g) g = gl;
   if ((rc = sjb::attn_noalloc_take_status(&sc)) != cudaSuccess)
     return launched(rc, "schedule status");
   if (sc)

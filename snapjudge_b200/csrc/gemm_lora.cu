@@ -105,7 +105,8 @@ int64_t sj_gemm_lora_workspace(const sj_lora_plan_info* info, int N, int K) {
     bad("bad projection shape");
     return -1;
   }
-  return (int64_t)info->M * info->rank * 2;
+  // the tcgen05 kernels' U (a slab for each block and sixteen ranks) or the others' [M, rank]
+  return std::max((int64_t)info->n_slabs * 256 * 32, (int64_t)info->M * info->rank * 2);
 }
 
 int sj_gemm_lora(const sj_gemm_lora_args* a, const sj_lora_plan_info* info, const int32_t* plan,
@@ -138,10 +139,14 @@ int sj_gemm_lora(const sj_gemm_lora_args* a, const sj_lora_plan_info* info, cons
   p.n_adapters = info->n_adapters;
   p.n_blocks = info->n_blocks;
   p.n_slabs = info->n_slabs;
+  p.max_slabs = info->max_slabs;
   p.rows = plan;
   p.blocks = plan + info->off_blocks;
   p.slabs = reinterpret_cast<const int2*>(plan + info->off_slabs);
-  const cudaError_t rc = sjb::gemm_lora_simt(p, workspace, static_cast<cudaStream_t>(stream));
+  const auto st = static_cast<cudaStream_t>(stream);
+  const bool tc = sjb::gemm_lora_tc_supported(p) && !(reinterpret_cast<uintptr_t>(workspace) & 15);
+  const cudaError_t rc =
+      tc ? sjb::gemm_lora_tc(p, workspace, st) : sjb::gemm_lora_simt(p, workspace, st);
   if (rc == cudaSuccess) return SJ_OK;
   sjb::set_last_error(std::string("snapjudge CUDA: gemm_lora: ") + cudaGetErrorString(rc));
   return SJ_ERR_CUDA;

@@ -12,11 +12,17 @@ struct GemmLora {
   bf16* C;
   int64_t ldx, ldc;
   int M, N, K, R, act, n_adapters;
-  int n_blocks, n_slabs;
+  int n_blocks, n_slabs, max_slabs;  // max_slabs: of any one block
   const int32_t* rows;    // plan: adapter of each row
   const int32_t* blocks;  // plan: [n_blocks + 1]
   const int2* slabs;      // plan: (adapter, sixteen)
 };
+
+// tcgen05 kernels (gemm_lora_tc.cu); U: n_slabs x 256 x 16 bf16 of workspace.
+bool gemm_lora_tc_supported(const GemmLora& p);
+cudaError_t gemm_lora_tc(const GemmLora& p, void* U, cudaStream_t st);
+// As attn_tc_take_status, for these kernels.
+cudaError_t gemm_lora_take_status(int* code);
 
 // Kernels on CUDA cores for every shape and alignment; U: M x R bf16 of workspace.
 cudaError_t gemm_lora_simt(const GemmLora& p, void* U, cudaStream_t st);

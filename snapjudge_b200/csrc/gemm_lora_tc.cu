@@ -1,0 +1,655 @@
+// gemm_lora_tc.cu — C = act(X W^T + bias + scale_a (X A_a^T) B_a^T) on tcgen05.
+//
+// Two kernels.  The first computes, for each block of 256 rows and each adapter
+// that a row of the block uses (the plan's slabs, 16 ranks each),
+// U = scale_a X A_a^T, rounded to bf16, with zeros in the rows that do not use
+// the adapter.  The second is a GEMM whose contraction runs over K and then over
+// the block's slabs: [X | U_1 U_2 ...] [W | B_1 B_2 ...]^T, so the adapters cost
+// one more tcgen05.mma (K = 16) for each slab of a tile and no pass over C.  A
+// row's zeros select its own adapter; 0 x NaN or infinity of another tenant's
+// adapter would reach it all the same, so a chunk of outputs that is not finite
+// is computed again from the row's own operands (repair).
+//
+// GEMM CTA: as gemm_tc.cu (warp 0 loads, warp 1 issues the MMAs, the other
+// warps write tile i while tile i + 1 is computed; TMEM double-buffered), in
+// the forms 256 x 256 by a pair of CTAs, and 128 x BN by one.  A slab is a
+// 128-row (B: BN-row) tile of 32 bytes, 32-byte swizzled; four of them take the
+// place of one 64-wide k-block in the ring of stages.  The second kernel is
+// launched while the first runs (programmatic dependent launch) and waits for
+// it before its first slab, after all of a tile's k-blocks are on their way.
+// Bounded waits and wind-down as in gemm_tc.cu.
+#include <algorithm>
+#include <atomic>
+
+#include "gemm_lora.cuh"
+#include "kernels.h"
+#include "tc_common.cuh"
+#include "tc_epilogue.cuh"
+#include "tc_host.h"
+
+namespace sjb {
+
+__device__ int g_gemm_lora_err;
+
+namespace {
+using namespace tc;
+
+constexpr int BM = 128, BK = 64;
+constexpr int SLAB_A = BM * 32;  // bytes of a slab of U for 128 rows
+constexpr int SLABS_PER_STAGE = 4;
+
+__device__ __forceinline__ void record_err(int code) { atomicCAS(&g_gemm_lora_err, 0, code); }
+
+// K-major tile of 16 bf16 (32 bytes) a row, 32-byte swizzle: 8-row groups 256 bytes apart
+__device__ __forceinline__ uint64_t desc_kmajor_sw32(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(256 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)6 << 61;
+  return d;
+}
+__device__ __forceinline__ void pdl_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// global writes of generic stores (the first kernel's U) before TMA reads of them
+__device__ __forceinline__ void fence_async_global() {
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
+// ---- U = scale_a X A_a^T -------------------------------------------------------
+// One CTA: 128 rows, up to 16 slabs (N = 256).  Thread 0 loads, thread 32 issues
+// the MMAs, all four warps write U (thread = row).
+constexpr int kShrinkStages = 4;
+
+__global__ void __launch_bounds__(128)
+    lora_shrink_kernel(const __grid_constant__ CUtensorMap mapX,
+                       const __grid_constant__ CUtensorMap mapA, const GemmLora p,
+                       bf16* __restrict__ U, int slabs_max, uint32_t tmem_cols) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kShrinkStages], empty[kShrinkStages], done;
+  __shared__ uint32_t tmem_sh;
+  __shared__ int issued_sh;
+  const int block = blockIdx.x >> 1, half = blockIdx.x & 1;
+  const int s0 = p.blocks[block] + 16 * (int)blockIdx.y;
+  const int ns = min(16, p.blocks[block + 1] - s0);
+  const int m0 = block * 256 + half * BM;
+  if (ns <= 0 || m0 >= p.M) return;  // block-uniform
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int stage_bytes = BM * BK * 2 + slabs_max * 16 * BK * 2;
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const int k_blocks = (p.K + BK - 1) / BK;
+  if (tid == 0) {
+    for (int s = 0; s < kShrinkStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&done, 1);
+    issued_sh = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) tmem_alloc(&tmem_sh, tmem_cols);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_sh;
+  // The GEMM's blocks may start now: not before this block has its TMEM, which
+  // they would take and keep while they wait for this kernel.
+  pdl_launch_dependents();
+  if (tid == 0) {
+    int kb = 0;
+    for (; kb < k_blocks; ++kb) {
+      const int st = kb % kShrinkStages;
+      if (kb >= kShrinkStages && !mbar_wait<true>(&empty[st], ((kb / kShrinkStages) - 1) & 1)) {
+        record_err(1);
+        break;
+      }
+      uint8_t* sx = smem + st * stage_bytes;
+      mbar_expect_tx(&full[st], BM * BK * 2 + ns * 16 * BK * 2);
+      tma_load_2d(sx, &mapX, &full[st], kb * BK, m0);
+      for (int s = 0; s < ns; ++s) {
+        const int2 sl = p.slabs[s0 + s];
+        tma_load_2d(sx + BM * BK * 2 + s * 16 * BK * 2, &mapA, &full[st], kb * BK,
+                    sl.x * p.R + 16 * sl.y);
+      }
+    }
+    issued_sh = kb;
+  } else if (tid == 32) {
+    const uint32_t idesc = idesc_bf16(BM, 16 * ns, false, false);
+    for (int kb = 0; kb < k_blocks; ++kb) {
+      const int st = kb % kShrinkStages;
+      if (!mbar_wait<true>(&full[st], (kb / kShrinkStages) & 1)) {
+        record_err(2);
+        break;
+      }
+      fence_after_sync();
+      const uint32_t a = smem_u32(smem + st * stage_bytes), b = a + BM * BK * 2;
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk)
+        mma_bf16(tmem, desc_kmajor_sw128(a + kk * 32), desc_kmajor_sw128(b + kk * 32), idesc,
+                 (kb | kk) != 0);
+      mma_commit(&empty[st]);
+    }
+    mma_commit(&done);
+  }
+  __syncwarp();
+  __syncthreads();
+  const bool ok = mbar_wait<true>(&done, 0);
+  if (tid == 0) {
+    if (!ok) record_err(3);
+    const int n = issued_sh;  // no copy outlives the block
+    for (int kb = max(0, n - kShrinkStages); kb < n; ++kb)
+      if (!mbar_wait<true>(&full[kb % kShrinkStages], (kb / kShrinkStages) & 1)) record_err(4);
+  }
+  fence_after_sync();
+  const int64_t row = (int64_t)m0 + tid;
+  const int mine = row < p.M ? p.rows[row] : -1;
+  const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+  if (ok) {
+    for (int s = 0; s < ns; ++s) {
+      const int2 sl = p.slabs[s0 + s];
+      uint32_t r[16];
+      tmem_ld16(tmem + lane_off + 16 * s, r);
+      tmem_ld_wait();
+      const float f = p.scale ? p.scale[sl.x] : 1.f;
+      const int live = sl.x == mine ? min(16, p.R - 16 * sl.y) : 0;
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = 2 * e < live ? f * __uint_as_float(r[2 * e]) : 0.f;
+        const float b = 2 * e + 1 < live ? f * __uint_as_float(r[2 * e + 1]) : 0.f;
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      uint4* u = reinterpret_cast<uint4*>(U + ((int64_t)(s0 + s) * 256 + half * BM + tid) * 16);
+      u[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      u[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    fence_after_sync();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// ---- the GEMM -----------------------------------------------------------------------
+template <int BN, bool PAIR>
+struct Cfg {
+  static constexpr int kEpiWarps = BN >= 64 ? 8 : 4;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr bool kStaged = BN >= 128;  // outputs through shared memory and TMA
+  static constexpr int kBRows = PAIR ? BN / 2 : BN;
+  static constexpr int kABytes = BM * BK * 2, kBBytes = kBRows * BK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kOutBytes = kStaged ? kEpiWarps * 2 * 32 * 128 : 0;
+  static constexpr int kStages = PAIR ? 5 : BN >= 256 ? 3 : BN >= 128 ? 5 : 8;
+  static constexpr int kSmem = kStages * kStageBytes + kOutBytes + 1024;
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static constexpr int kTileM = PAIR ? 2 * BM : BM;
+};
+
+// 32 outputs of a row whose accumulators v are not all finite: those that are
+// not are computed again from the row's own operands (unless the row's input is
+// not finite: then the tile's values are its own), then bias and activation.
+__device__ __noinline__ void repair(const GemmLora& p, int64_t row, int n0, float* v) {
+  const bf16* x = p.X + row * p.ldx;
+  bool fine = true;
+  for (int k = 0; k < p.K; ++k) fine = fine && fabsf(__bfloat162float(x[k])) <= 3.4e38f;
+  const int a = p.rows[row];
+  for (int j = 0; j < 32 && n0 + j < p.N; ++j) {
+    if (fine && !(fabsf(v[j]) <= 3.4e38f)) {
+      const bf16* w = p.W + (int64_t)(n0 + j) * p.K;
+      float s = 0.f;
+      for (int k = 0; k < p.K; ++k) s += __bfloat162float(x[k]) * __bfloat162float(w[k]);
+      if (a >= 0) {
+        const bf16* b = p.B + ((int64_t)a * p.N + n0 + j) * p.R;
+        for (int r = 0; r < p.R; ++r) {
+          const bf16* ar = p.A + ((int64_t)a * p.R + r) * p.K;
+          float u = 0.f;
+          for (int k = 0; k < p.K; ++k) u += __bfloat162float(x[k]) * __bfloat162float(ar[k]);
+          if (p.scale) u *= p.scale[a];
+          s += __bfloat162float(__float2bfloat16(u)) * __bfloat162float(b[r]);
+        }
+      }
+      v[j] = s;
+    }
+    if (p.bias) v[j] += p.bias[n0 + j];
+    if (p.act == ACT_GELU) v[j] = gelu_erf(v[j]);
+    else if (p.act == ACT_RELU) v[j] = v[j] < 0.f ? 0.f : v[j];
+  }
+}
+
+// 32 accumulators of a row -> outputs (bias, activation).  Columns past N hold
+// whatever the tile computed there and are not stored.
+__device__ __forceinline__ void finish32(const GemmLora& p, const uint32_t (&r)[32], int64_t row,
+                                         int n0, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+  float t = 0.f;  // stays 0 while every value is finite
+#pragma unroll
+  for (int j = 0; j < 32; ++j) t = fmaf(v[j], 0.f, t);
+  if (t != 0.f && row < p.M) {
+    float again[32];  // a copy, so that v stays in registers
+#pragma unroll
+    for (int j = 0; j < 32; ++j) again[j] = v[j];
+    repair(p, row, n0, again);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = again[j];
+    return;
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2)
+      if (n0 + j < p.N) {
+        const float2 b = *reinterpret_cast<const float2*>(p.bias + n0 + j);
+        v[j] += b.x;
+        v[j + 1] += b.y;
+      }
+  }
+  if (p.act == ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float2 g = unpk2(gelu2(v[j], v[j + 1]));
+      v[j] = g.x;
+      v[j + 1] = g.y;
+    }
+  } else if (p.act == ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];
+  }
+}
+
+template <int BN, bool PAIR>
+__global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
+    gemm_lora_kernel(const __grid_constant__ CUtensorMap mapX,
+                     const __grid_constant__ CUtensorMap mapW,
+                     const __grid_constant__ CUtensorMap mapU,
+                     const __grid_constant__ CUtensorMap mapB,
+                     const __grid_constant__ CUtensorMap mapC, const __grid_constant__ GemmLora p,
+                     int n_tiles) {
+  using F = Cfg<BN, PAIR>;
+  constexpr int STAGES = F::kStages;
+  constexpr uint32_t IDESC = idesc_bf16(F::kTileM, BN, false, false);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], tfull_bar[2], tempty_bar[2], drain_bar;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ volatile int abort_sh;
+
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+  const int units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  const int m_tiles = (p.M + F::kTileM - 1) / F::kTileM;
+  const int num_tiles = m_tiles * n_tiles;
+  const int k_blocks = (p.K + BK - 1) / BK;
+  // the plan's block of 256 rows that holds tile row mt
+  auto block_of = [](int mt) { return PAIR ? mt : mt >> 1; };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], F::kEpiWarps * (PAIR ? 2 : 1));
+    }
+    mbar_init(&drain_bar, 1);
+    abort_sh = 0;
+    fence_barrier_init();
+    tma_prefetch(&mapX);
+    tma_prefetch(&mapW);
+    tma_prefetch(&mapU);
+    tma_prefetch(&mapB);
+    if (F::kStaged) tma_prefetch(&mapC);
+  }
+  if (warp == 1) {
+    if (PAIR) tmem_alloc_pair(&tmem_base_sh, F::kTmemCols);
+    else tmem_alloc(&tmem_base_sh, F::kTmemCols);
+  }
+  fence_before_sync();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem_base = tmem_base_sh;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- loads (both CTAs of a pair) ----------------
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool u_ready = false;
+    for (int t = unit; t < num_tiles && !abort_sh; t += units) {
+      const int mt = t / n_tiles, nb = t % n_tiles;
+      const int m0 = mt * F::kTileM + (int)rank * BM;
+      const int n0 = nb * BN + (int)rank * F::kBRows;
+      const int blk = block_of(mt);
+      const int s0 = p.blocks[blk], s1 = p.blocks[blk + 1];
+      // first row of this CTA's 128 within a slab of U
+      const int u_row = PAIR ? (int)rank * BM : (mt & 1) * BM;
+      const int steps = k_blocks + (s1 - s0 + SLABS_PER_STAGE - 1) / SLABS_PER_STAGE;
+      for (int kb = 0; kb < steps; ++kb) {
+        if (!mbar_wait<true>(&empty_bar[stage], phase ^ 1)) {
+          record_err(11);
+          abort_sh = 1;
+          break;
+        }
+        uint8_t* sa = smem + stage * F::kStageBytes;
+        uint8_t* sb = sa + F::kABytes;
+        const int sl0 = s0 + (kb - k_blocks) * SLABS_PER_STAGE;
+        const int ns = kb < k_blocks ? 0 : min(SLABS_PER_STAGE, s1 - sl0);
+        const uint32_t bytes =
+            kb < k_blocks ? F::kStageBytes : ns * (SLAB_A + F::kBRows * 32);
+        if (ns > 0 && !u_ready) {
+          pdl_wait();
+          fence_async_global();
+          u_ready = true;
+        }
+        if (PAIR) {
+          // both CTAs' bytes are counted on rank 0's barrier
+          const uint32_t bar0 = mapa_shared(smem_u32(&full_bar[stage]), 0);
+          if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * bytes);
+          if (ns == 0) {
+            tma_load_2d_pair(sa, &mapX, bar0, kb * BK, m0);
+            tma_load_2d_pair(sb, &mapW, bar0, kb * BK, n0);
+          }
+          for (int s = 0; s < ns; ++s) {
+            const int2 sl = p.slabs[sl0 + s];
+            tma_load_2d_pair(sa + s * SLAB_A, &mapU, bar0, 0, (sl0 + s) * 256 + u_row);
+            tma_load_2d_pair(sb + s * F::kBRows * 32, &mapB, bar0, 16 * sl.y, sl.x * p.N + n0);
+          }
+        } else {
+          mbar_expect_tx(&full_bar[stage], bytes);
+          if (ns == 0) {
+            tma_load_2d(sa, &mapX, &full_bar[stage], kb * BK, m0);
+            tma_load_2d(sb, &mapW, &full_bar[stage], kb * BK, n0);
+          }
+          for (int s = 0; s < ns; ++s) {
+            const int2 sl = p.slabs[sl0 + s];
+            tma_load_2d(sa + s * SLAB_A, &mapU, &full_bar[stage], 0, (sl0 + s) * 256 + u_row);
+            tma_load_2d(sb + s * F::kBRows * 32, &mapB, &full_bar[stage], 16 * sl.y,
+                        sl.x * p.N + n0);
+          }
+        }
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!u_ready) pdl_wait();  // this kernel's end implies the first one's
+    if (!PAIR || rank == 0) {
+      for (int i = 0; i < STAGES && i < issued; ++i) {
+        if (--stage < 0) { stage = STAGES - 1; phase ^= 1; }
+        if (!mbar_wait<true>(&full_bar[stage], phase)) record_err(12);
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---------------- MMAs (rank 0 of a pair) ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    int local = 0;
+    for (int t = unit; t < num_tiles && !abort_sh; t += units, ++local) {
+      const int b = local & 1;
+      const int blk = block_of(t / n_tiles);
+      const int n_slabs = p.blocks[blk + 1] - p.blocks[blk];
+      if (!mbar_wait<true>(&tempty_bar[b], ((local >> 1) & 1) ^ 1)) {
+        record_err(13);
+        abort_sh = 1;
+        break;
+      }
+      fence_after_sync();
+      const uint32_t d = tmem_base + b * BN;
+      const int steps = k_blocks + (n_slabs + SLABS_PER_STAGE - 1) / SLABS_PER_STAGE;
+      for (int kb = 0; kb < steps; ++kb) {
+        if (!mbar_wait<true>(&full_bar[stage], phase)) {
+          record_err(14);
+          abort_sh = 1;
+          break;
+        }
+        fence_after_sync();
+        const uint32_t a_addr = smem_u32(smem + stage * F::kStageBytes);
+        const uint32_t b_addr = a_addr + F::kABytes;
+        if (kb < k_blocks) {
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            const uint64_t ad = desc_kmajor_sw128(a_addr + kk * 32);
+            const uint64_t bd = desc_kmajor_sw128(b_addr + kk * 32);
+            if (PAIR) mma_bf16_pair(d, ad, bd, IDESC, (kb | kk) != 0);
+            else mma_bf16(d, ad, bd, IDESC, (kb | kk) != 0);
+          }
+        } else {
+          const int ns = min(SLABS_PER_STAGE, n_slabs - (kb - k_blocks) * SLABS_PER_STAGE);
+          for (int s = 0; s < ns; ++s) {
+            const uint64_t ad = desc_kmajor_sw32(a_addr + s * SLAB_A);
+            const uint64_t bd = desc_kmajor_sw32(b_addr + s * F::kBRows * 32);
+            if (PAIR) mma_bf16_pair(d, ad, bd, IDESC, 1u);
+            else mma_bf16(d, ad, bd, IDESC, 1u);
+          }
+        }
+        if (PAIR) mma_commit_pair(&empty_bar[stage], 0x3);
+        else mma_commit(&empty_bar[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      if (PAIR) mma_commit_pair(&tfull_bar[b], 0x3);
+      else mma_commit(&tfull_bar[b]);
+    }
+    if (PAIR) mma_commit_pair(&drain_bar, 0x1);
+    else mma_commit(&drain_bar);
+    if (!mbar_wait<true>(&drain_bar, 0)) record_err(15);
+  } else if (warp >= 2) {
+    // ---------------- epilogue ----------------
+    constexpr int PARTS = F::kEpiWarps / 4;  // warps of a row quarter share its columns
+    const int q = warp & 3, hf = (warp - 2) >> 2;
+    uint8_t* stg = smem + STAGES * F::kStageBytes + (warp - 2) * 2 * 32 * 128;
+    int sbuf = 0, local = 0;
+    for (int t = unit; t < num_tiles; t += units, ++local) {
+      const int b = local & 1;
+      const int row0 = (t / n_tiles) * F::kTileM + (int)rank * BM + q * 32;
+      const int64_t row = row0 + lane;
+      const int col0 = (t % n_tiles) * BN;
+      int ok = 1;
+      if (lane == 0) ok = mbar_wait<true>(&tfull_bar[b], (local >> 1) & 1) ? 1 : 0;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok || abort_sh) {
+        if (lane == 0 && !ok) { record_err(16); abort_sh = 1; }
+        break;
+      }
+      fence_after_sync();
+      const uint32_t tacc = tmem_base + ((uint32_t)(q * 32) << 16) + b * BN;
+      uint32_t r[32];
+      if constexpr (F::kStaged) {
+#pragma unroll 1
+        for (int c = hf * BN / PARTS; c < (hf + 1) * BN / PARTS; c += 64) {
+          if (col0 + c >= p.N) break;
+          if (lane == 0) bulk_wait_read<1>();  // this buffer's previous store has read it
+          __syncwarp();
+          uint8_t* rowp = stg + sbuf * (32 * 128) + lane * 128;
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            float v[32];
+            tmem_ld32(tacc + c + 32 * k2, r);
+            tmem_ld_wait();
+            finish32(p, r, row, col0 + c + 32 * k2, v);
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * u + 2 * e], v[8 * u + 2 * e + 1]);
+                w[e] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              *reinterpret_cast<uint4*>(rowp + (((4 * k2 + u) ^ (lane & 7)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&mapC, stg + sbuf * (32 * 128), col0 + c, row0);
+            bulk_commit();
+          }
+          sbuf ^= 1;
+        }
+      } else {
+#pragma unroll 1
+        for (int c = hf * BN / PARTS; c < (hf + 1) * BN / PARTS; c += 32) {
+          tmem_ld32(tacc + c, r);
+          tmem_ld_wait();
+          if (row >= p.M) continue;
+          float v[32];
+          finish32(p, r, row, col0 + c, v);
+          bf16* out = p.C + row * p.ldc + col0 + c;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (col0 + c + 8 * u >= p.N) break;  // N is a multiple of 8
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * u + 2 * e], v[8 * u + 2 * e + 1]);
+              w[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            reinterpret_cast<uint4*>(out)[u] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      // hand the accumulator back to the MMA thread (rank 0's barrier in a pair)
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[b]), 0));
+        else mbar_arrive(&tempty_bar[b]);
+      }
+    }
+    if (F::kStaged && lane == 0) bulk_wait_all();
+  }
+
+  fence_before_sync();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    fence_after_sync();
+    if (PAIR) tmem_dealloc_pair(tmem_base, F::kTmemCols);
+    else tmem_dealloc(tmem_base, F::kTmemCols);
+  }
+}
+
+// 2-D map of rows of 16 bf16 (32 bytes), 32-byte swizzle
+bool make_map_slab(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows,
+                   uint64_t row_bytes, uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || (row_bytes & 15)) return false;
+  cuuint64_t dims[2] = {inner, rows};
+  cuuint64_t strides[1] = {row_bytes};
+  cuuint32_t box[2] = {16, box_rows};
+  cuuint32_t es[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, bool PAIR>
+cudaError_t launch_gemm(const GemmLora& p, const bf16* U, cudaStream_t st) {
+  using F = Cfg<BN, PAIR>;
+  static std::atomic<uint64_t> attr_done{0};  // per device ordinal
+  auto kernel = gemm_lora_kernel<BN, PAIR>;
+  if (cudaError_t rc = ensure_smem_attr(kernel, F::kSmem, attr_done)) return rc;
+  CUtensorMap mx, mw, mu, mb, mc;
+  if (!make_map_bf16(&mx, p.X, p.K, p.M, (uint64_t)p.ldx * 2, BK, BM) ||
+      !make_map_bf16(&mw, p.W, p.K, p.N, (uint64_t)p.K * 2, BK, F::kBRows) ||
+      !make_map_bf16(&mc, p.C, p.N, p.M, (uint64_t)p.ldc * 2, 64, 32))
+    return cudaErrorInvalidValue;
+  if (p.n_slabs == 0) {
+    mu = mb = mx;  // never read
+  } else if (!make_map_slab(&mu, U, 16, (uint64_t)p.n_slabs * 256, 32, BM) ||
+             !make_map_slab(&mb, p.B, p.R, (uint64_t)p.n_adapters * p.N, (uint64_t)p.R * 2,
+                            F::kBRows)) {
+    return cudaErrorInvalidValue;
+  }
+  const int n_tiles = (p.N + BN - 1) / BN;
+  const int64_t tiles = ((int64_t)p.M + F::kTileM - 1) / F::kTileM * n_tiles;
+  if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const int units = (int)std::min<int64_t>(tiles, PAIR ? sm_count() / 2 : sm_count());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(PAIR ? 2 * units : units, 1, 1);
+  cfg.blockDim = dim3(F::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = F::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (PAIR) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 2;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (p.n_slabs > 0) {  // overlaps the first kernel
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, mu, mb, mc, p, n_tiles);
+}
+
+cudaError_t launch_shrink(const GemmLora& p, bf16* U, cudaStream_t st) {
+  const int slabs = std::min(16, p.max_slabs);
+  const int smem = kShrinkStages * (BM * BK * 2 + slabs * 16 * BK * 2) + 1024;
+  static std::atomic<uint64_t> attr_done{0};
+  constexpr int most = kShrinkStages * (BM * BK * 2 + 16 * 16 * BK * 2) + 1024;
+  if (cudaError_t rc = ensure_smem_attr(lora_shrink_kernel, most, attr_done)) return rc;
+  CUtensorMap mx, ma;
+  if (!make_map_bf16(&mx, p.X, p.K, p.M, (uint64_t)p.ldx * 2, BK, BM) ||
+      !make_map_bf16(&ma, p.A, p.K, (uint64_t)p.n_adapters * p.R, (uint64_t)p.K * 2, BK, 16))
+    return cudaErrorInvalidValue;
+  uint32_t cols = 32;
+  while ((int)cols < 16 * slabs) cols *= 2;
+  const int groups = (p.max_slabs + 15) / 16;
+  if (groups > 65535) return cudaErrorInvalidConfiguration;
+  lora_shrink_kernel<<<dim3(2 * p.n_blocks, groups), 128, smem, st>>>(mx, ma, p, U, slabs, cols);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+// 16-byte rows and addresses; everything else goes to the CUDA-core kernels.
+bool gemm_lora_tc_supported(const GemmLora& p) {
+  auto on = [](const void* q, int a) { return !(reinterpret_cast<uintptr_t>(q) & (a - 1)); };
+  if (p.K < 8 || p.K % 8 || p.N % 8 || p.ldx % 8 || p.ldc % 8) return false;
+  if (!on(p.X, 16) || !on(p.W, 16) || !on(p.C, 16) || !on(p.bias, 8)) return false;
+  if (p.n_slabs > 0 && (p.R % 8 || !on(p.A, 16) || !on(p.B, 16))) return false;
+  return (int64_t)p.n_adapters * p.N <= 0x7fffffff && (int64_t)p.n_adapters * p.R <= 0x7fffffff;
+}
+
+cudaError_t gemm_lora_tc(const GemmLora& p, void* U, cudaStream_t st) {
+  bf16* u = static_cast<bf16*>(U);
+  if (p.n_slabs > 0)
+    if (cudaError_t rc = launch_shrink(p, u, st)) return rc;
+  if (p.M >= 2048) return launch_gemm<256, true>(p, u, st);
+  const int64_t mt = (p.M + BM - 1) / BM;
+  const int sms = sm_count();
+  if (mt * ((p.N + 255) / 256) >= sms) return launch_gemm<256, false>(p, u, st);
+  if (mt * ((p.N + 127) / 128) >= sms) return launch_gemm<128, false>(p, u, st);
+  if (mt * ((p.N + 63) / 64) >= sms) return launch_gemm<64, false>(p, u, st);
+  return launch_gemm<32, false>(p, u, st);
+}
+
+cudaError_t gemm_lora_take_status(int* code) {
+  int v = 0;
+  cudaError_t rc = cudaMemcpyFromSymbol(&v, g_gemm_lora_err, sizeof(int));
+  if (rc == cudaSuccess && v != 0) {
+    const int zero = 0;
+    rc = cudaMemcpyToSymbol(g_gemm_lora_err, &zero, sizeof(int));
+  }
+  *code = v;
+  return rc;
+}
+
+}  // namespace sjb

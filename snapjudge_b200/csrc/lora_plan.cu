@@ -36,6 +36,7 @@ int make_plan(const int32_t* cu, int B, const int32_t* ids, int n_adapters, int 
   const int nb = (int)(((long long)M + 255) / 256);
   std::vector<int32_t> slabs, first((size_t)nb + 1, 0);
   std::vector<int> seen((size_t)n_adapters, -1);  // last block that listed the adapter
+  int32_t most = 0;
   for (int k = 0, b = 0; k < nb; ++k) {
     const int r1 = std::min<long long>(M, 256ll * (k + 1));
     while (b > 0 && cu[b] > 256 * k) --b;
@@ -51,12 +52,14 @@ int make_plan(const int32_t* cu, int B, const int32_t* ids, int n_adapters, int 
     }
     if (slabs.size() / 2 > 0x7fffff) return bad("the batch needs too many adapter blocks");
     first[k + 1] = (int32_t)(slabs.size() / 2);
+    most = std::max(most, first[k + 1] - first[k]);
   }
   info->M = M;
   info->rank = rank;
   info->n_adapters = n_adapters;
   info->n_blocks = nb;
   info->n_slabs = (int32_t)(slabs.size() / 2);
+  info->max_slabs = most;
   info->off_blocks = ((long long)M + 3) / 4 * 4;
   info->off_slabs = info->off_blocks + ((long long)nb + 1 + 3) / 4 * 4;
   info->plan_len = info->off_slabs + (long long)slabs.size();

@@ -1,0 +1,122 @@
+// tc_epilogue.cuh — arithmetic of the tcgen05 GEMMs' epilogues: packed fp32
+// pairs, the erf GELU, bias and activation, bf16 stores.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace sjb {
+namespace tc {
+
+// ---- GEGLU gate on column pairs, packed fp32 (fma/mul .f32x2) ----
+// erf by Abramowitz & Stegun, Handbook of Mathematical Functions, eq. 7.1.26:
+//   erfc(z) = (a1 t + a2 t^2 + a3 t^3 + a4 t^4 + a5 t^5) exp(-z^2),
+//   t = 1 / (1 + p z), z >= 0, |error| <= 1.5e-7,
+// with z = |x| / sqrt(2), so 1 - Phi(|x|) = erfc(z) / 2 and
+//   gelu(x) = x Phi(x) = relu(x) - |x| (1 - Phi(|x|)).
+// The reciprocal and exponential are the approximate hardware ones (relative
+// error ~2^-22); the gate is then rounded to bf16, so the result matches the
+// erf GELU to within one bf16 rounding step.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pk2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpk2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 splat2(float a) { return pk2(a, a); }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (gelu(ga), gelu(gb)), packed
+__device__ __forceinline__ f32x2 gelu2(float ga, float gb) {
+  constexpr float kP = 0.3275911f * 0.70710678118654752f;  // p / sqrt(2)
+  // -a_i / 2: the polynomial comes out as -erfc(z) / 2 before the exponential
+  constexpr float kA1 = -0.5f * 0.254829592f, kA2 = 0.5f * 0.284496736f,
+                  kA3 = -0.5f * 1.421413741f, kA4 = 0.5f * 1.453152027f,
+                  kA5 = -0.5f * 1.061405429f;
+  constexpr float kE = -0.5f * 1.4426950408889634f;  // -z^2 log2(e) = x^2 * kE
+  const f32x2 ax = pk2(fabsf(ga), fabsf(gb));
+  const float2 d = unpk2(fma2(ax, splat2(kP), splat2(1.f)));
+  const f32x2 t = pk2(rcp_approx(d.x), rcp_approx(d.y));
+  f32x2 p = fma2(t, splat2(kA5), splat2(kA4));
+  p = fma2(t, p, splat2(kA3));
+  p = fma2(t, p, splat2(kA2));
+  p = fma2(t, p, splat2(kA1));
+  p = mul2(p, t);
+  const f32x2 g = pk2(ga, gb);
+  const float2 e = unpk2(mul2(mul2(g, g), splat2(kE)));
+  const f32x2 h = mul2(p, pk2(ex2_approx(e.x), ex2_approx(e.y)));  // -(1 - Phi(|x|))
+  return fma2(ax, h, pk2(fmaxf(ga, 0.f), fmaxf(gb, 0.f)));
+}
+
+// The STORE epilogue's 32 accumulator values: + bias[0..32) (when given), then
+// the activation, chosen once per call so that the unrolled loop holds one
+// activation's code; GELU is the GEGLU gate's erf approximation above.
+template <int ACT>
+__device__ __forceinline__ void bias_act32(const uint32_t (&r)[32], const float* bias, float* v) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float a0 = __uint_as_float(r[j]), a1 = __uint_as_float(r[j + 1]);
+    if (bias) {
+      const float2 bb = *reinterpret_cast<const float2*>(bias + j);
+      a0 += bb.x;
+      a1 += bb.y;
+    }
+    if (ACT == ACT_GELU) {
+      const float2 g = unpk2(gelu2(a0, a1));
+      a0 = g.x;
+      a1 = g.y;
+    } else if (ACT == ACT_RELU) {
+      a0 = fmaxf(a0, 0.f);
+      a1 = fmaxf(a1, 0.f);
+    }
+    v[j] = a0;
+    v[j + 1] = a1;
+  }
+}
+__device__ __forceinline__ void bias_act32(const uint32_t (&r)[32], const float* bias, int act,
+                                           float* v) {
+  if (act == ACT_GELU) bias_act32<ACT_GELU>(r, bias, v);
+  else if (act == ACT_RELU) bias_act32<ACT_RELU>(r, bias, v);
+  else bias_act32<ACT_NONE>(r, bias, v);
+}
+
+__device__ __forceinline__ void store_bf16x32(bf16* dst, const float* v) {
+  uint4* d = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      __nv_bfloat162 h = __floats2bfloat162_rn(v[q * 8 + 2 * e], v[q * 8 + 2 * e + 1]);
+      w[e] = *reinterpret_cast<uint32_t*>(&h);
+    }
+    d[q] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+}  // namespace tc
+}  // namespace sjb
