@@ -77,7 +77,9 @@ int sj_attn_masked(const sj_attn_masked_args* a, const sj_attn_plan_info* info,
   const int64_t need = sj_attn_masked_workspace(info, a->H, a->Hkv, a->Dh);
   if (workspace_bytes < need || (need > 0 && !workspace)) return bad("the workspace is too small");
   sjb::AttnMasked p = sjb::attn_masked_params(*a, *info, plan);
-  const cudaError_t rc = sjb::attn_masked_simt(p, static_cast<cudaStream_t>(stream));
+  const auto st = static_cast<cudaStream_t>(stream);
+  const cudaError_t rc = sjb::attn_masked_tc_supported(p) ? sjb::attn_masked_tc(p, st)
+                                                          : sjb::attn_masked_simt(p, st);
   if (rc == cudaSuccess) return SJ_OK;
   sjb::set_last_error(std::string("snapjudge CUDA: attn_masked: ") + cudaGetErrorString(rc));
   return SJ_ERR_CUDA;

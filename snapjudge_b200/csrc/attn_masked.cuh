@@ -17,6 +17,7 @@ struct AttnMasked {
   int rel_max;
   const float* slopes;        // [H] or null
   int n_rows, n_keys, n_items;
+  bool rows_consecutive;      // query row r is key row r (no q_rows)
   const int4* rows;           // plan: 2 x int4 for each query row
   const int4* items;          // plan: one for each query tile
   const int32_t* tiles;       // plan: key tiles
@@ -44,6 +45,7 @@ inline AttnMasked attn_masked_params(const sj_attn_masked_args& a, const sj_attn
   p.n_rows = info.n_rows;
   p.n_keys = info.n_keys;
   p.n_items = info.n_items;
+  p.rows_consecutive = info.n_rows == info.n_keys;
   p.rows = reinterpret_cast<const int4*>(plan);
   p.items = reinterpret_cast<const int4*>(plan + info.off_items);
   p.tiles = plan + info.off_tiles;
@@ -62,7 +64,7 @@ __device__ __forceinline__ float attn_score(const AttnMasked& p, const float* re
 
 // One query row of one head by one warp, online over 32 keys at a time; lane l
 // gets the output's dimensions l, l + 32, l + 64, l + 96 in o.
-__device__ __noinline__ void attn_masked_row(const AttnMasked& p, int row, int h, int lane,
+static __device__ __noinline__ void attn_masked_row(const AttnMasked& p, int row, int h, int lane,
                                              float (&o)[4]) {
   const int4 r0 = p.rows[2 * (int64_t)row], r1 = p.rows[2 * (int64_t)row + 1];
   const int pos = r0.x, a0 = r0.y, na = r0.z - r0.y, b0 = r0.w, nk = na + (r1.x - r0.w);
@@ -109,5 +111,10 @@ __device__ __noinline__ void attn_masked_row(const AttnMasked& p, int row, int h
 }
 
 cudaError_t attn_masked_simt(const AttnMasked& p, cudaStream_t st);
+// tcgen05 kernel (attn_masked_tc.cu)
+bool attn_masked_tc_supported(const AttnMasked& p);
+cudaError_t attn_masked_tc(const AttnMasked& p, cudaStream_t st);
+// As attn_tc_take_status, for this kernel.
+cudaError_t attn_masked_take_status(int* code);
 
 }  // namespace sjb

@@ -1,0 +1,600 @@
+// attn_masked_tc.cu — attention with score caps, distance biases and document /
+// prefix masks on tcgen05 (head_dim 64 and 128).
+//
+// Work items are the plan's tiles of 128 query rows, for one head each, longest
+// first; each walks the 64-key tiles that its rows need.  A CTA of 128 threads
+// (thread = query row = TMEM lane) is a whole pipeline: thread 0 issues the
+// MMAs, thread 96 the TMA loads (Q once per item, K and V tiles through a
+// two-stage ring that runs on across items), every thread computes its row's
+// softmax:
+//   S = Q K^T into TMEM -> registers; x = cap tanh(scale s / cap) + bias, in
+//   units of log2; keys outside the row's two intervals -inf (tiles that every
+//   row sees whole skip this); p = 2^(x - m), m the row's reference maximum;
+//   P (bf16 pairs) over S in TMEM; O += P V.
+// Several such CTAs share an SM (4 at head_dim 64, 2 at 128), so that one's
+// softmax runs beside another's MMAs.
+// The reference maximum moves only when a tile's maximum exceeds it by 2^8; the
+// row's O in TMEM and its sum are then rescaled.  Sums and O are fp32; P is
+// rounded to bf16 because V is bf16 and the MMA takes one type.
+// Table biases of consecutive query rows: the 191 distances of a (query, key)
+// tile pair are staged in shared memory one tile ahead; the row reads entry
+// c - r + 127 for its column c, without bank conflicts.
+// A masked key has p = 0, and 0 x NaN or infinity of its V would still reach
+// the row: a row whose output is not finite is computed again over its visible
+// keys alone (attn_masked_row).
+// Waits are bounded and failures carried to the next block-wide barrier, as in
+// attn_tc.cu.
+#include <algorithm>
+#include <atomic>
+
+#include "attn_masked.cuh"
+#include "kernels.h"
+#include "tc_common.cuh"
+#include "tc_epilogue.cuh"
+#include "tc_host.h"
+
+namespace sjb {
+
+__device__ int g_attn_masked_err;
+
+namespace {
+using namespace tc;
+
+constexpr int QT = 128, KT = 64;
+constexpr int kThreads = 128;
+constexpr int KV_STAGES = 2;
+constexpr int CHUNK = 32;  // work items decoded at a time
+constexpr float kRescaleLog2 = 8.f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int WIN = QT + KT;  // staged distances (191 used)
+
+enum Rel { REL_NONE = 0, REL_WINDOW = 1, REL_DIRECT = 2 };
+
+template <int DH>
+struct Shape {
+  static constexpr int kCtas = DH == 64 ? 4 : 2;  // per SM
+  static constexpr int kQBytes = QT * DH * 2, kKvBytes = KT * DH * 2;
+  static constexpr int kSmem = kQBytes + KV_STAGES * 2 * kKvBytes + 1024;
+  static constexpr uint32_t kTmemCols = DH == 64 ? 128 : 256;
+  static constexpr uint32_t kColS = 0, kColO = KT;  // P in columns [0, 32), over S
+};
+
+__device__ __forceinline__ void record_err(int code) { atomicCAS(&g_attn_masked_err, 0, code); }
+
+__device__ __forceinline__ float tanh_mufu(float x) {
+  float y;
+  asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// A bias in units of log2.  A finite one stays finite (a bias of the type's
+// lowest value is a score like any other), -inf stays -inf.
+__device__ __forceinline__ float bias_log2(float b) {
+  const float v = b * kLog2e;
+  return fabsf(b) <= 3.402823466e38f ? fminf(fmaxf(v, -3.402823466e38f), 3.402823466e38f) : v;
+}
+// bits [a, b) of a 64-bit word, a and b clamped to 0 .. 64
+__device__ __forceinline__ uint64_t bit_range(int a, int b) {
+  a = max(a, 0);
+  b = min(b, 64);
+  if (a >= b) return 0;
+  return (~0ull >> (64 - (b - a))) << a;
+}
+
+struct __align__(16) Item {
+  int row0, rows, tile0, n_tiles;
+  int h, first, pos0, pad;  // head, first key-tile entry, position of the first row
+};
+
+template <int DH, bool RAW, bool CAP, int REL, bool SLOPE>
+__global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
+    attn_masked_tc_kernel(const __grid_constant__ CUtensorMap mapQ,
+                          const __grid_constant__ CUtensorMap mapK,
+                          const __grid_constant__ CUtensorMap mapV,
+                          const __grid_constant__ AttnMasked p, int n_work) {
+  using F = Shape<DH>;
+  constexpr uint32_t IDESC_S = idesc_bf16(QT, KT, false, false);
+  constexpr uint32_t IDESC_O = idesc_bf16(QT, 64, false, true);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t q_full, kv_full[KV_STAGES], s_full, pv_done, drain;
+  __shared__ Item items[2][CHUNK];  // this CTA's work items, chunk c in items[c & 1]
+  __shared__ uint32_t tmem_sh;
+  __shared__ float win[REL == REL_WINDOW ? 2 : 1][REL == REL_WINDOW ? WIN : 1];
+  __shared__ struct {
+    int lk, lj;          // loader: next K/V tile to load: item lk, tile lj
+    uint32_t kv_issued, q_issued;
+    int q_item;          // item whose Q is in the buffer or on its way
+    uint32_t kv_done, q_done, s_issued;  // thread 0
+  } ls;
+
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + F::kQBytes;  // stage s: K, then V
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool leader = tid == 0, loader = tid == 96;
+  const int group = p.H / p.Hkv;
+  const int cnt =
+      n_work > (int)blockIdx.x ? (n_work - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+
+  auto decode_chunk = [&](int c) {
+    const int k = c * CHUNK + tid;
+    if (tid < CHUNK && k < cnt) {
+      const int w = (int)blockIdx.x + k * (int)gridDim.x;
+      const int4 v = p.items[w / p.H];
+      Item it;
+      it.row0 = v.x;
+      it.rows = v.y;
+      it.tile0 = v.z;
+      it.n_tiles = v.w;
+      it.h = w % p.H;
+      it.first = v.w > 0 ? p.tiles[v.z] : 0;
+      it.pos0 = p.rows[2 * (int64_t)v.x].x;
+      it.pad = 0;
+      items[c & 1][tid] = it;
+    }
+  };
+  if (leader) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < KV_STAGES; ++s) mbar_init(&kv_full[s], 1);
+    mbar_init(&s_full, 1);
+    mbar_init(&pv_done, 1);
+    mbar_init(&drain, 1);
+    fence_barrier_init();
+    tma_prefetch(&mapQ);
+    tma_prefetch(&mapK);
+    tma_prefetch(&mapV);
+    ls.lk = ls.lj = 0;
+    ls.kv_issued = ls.kv_done = ls.q_issued = ls.q_done = ls.s_issued = 0;
+    ls.q_item = -1;
+  }
+  if (warp == 0) tmem_alloc(&tmem_sh, F::kTmemCols);
+  decode_chunk(0);
+  decode_chunk(1);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_sh;
+
+  auto item_at = [&](int k) -> const Item& { return items[(k / CHUNK) & 1][k % CHUNK]; };
+  auto first_key = [](int entry) { return entry < 0 ? ~entry : entry; };
+  auto kv_out = [&]() { return *reinterpret_cast<volatile uint32_t*>(&ls.kv_issued); };
+  auto q_out_item = [&]() { return *reinterpret_cast<volatile int*>(&ls.q_item); };
+
+  // ---- loads (thread 96) ----
+  auto issue_kv = [&](uint32_t released, int chunk_hi) {
+    const int k_end = min(cnt, (chunk_hi + 1) * CHUNK);
+    while (ls.kv_issued < released + KV_STAGES && ls.lk < k_end) {
+      const Item& it = item_at(ls.lk);
+      if (it.n_tiles <= 0) {
+        ++ls.lk;
+        ls.lj = 0;
+        continue;
+      }
+      const int stage = ls.kv_issued % KV_STAGES;
+      const int k0 = first_key(ls.lj == 0 ? it.first : p.tiles[it.tile0 + ls.lj]);
+      const int x = it.h / group * DH;
+      uint8_t* dst = sKV + stage * 2 * F::kKvBytes;
+      mbar_expect_tx(&kv_full[stage], 2 * F::kKvBytes);
+#pragma unroll
+      for (int d = 0; d < DH; d += 64) {
+        tma_load_2d(dst + d * KT * 2, &mapK, &kv_full[stage], x + d, k0);
+        tma_load_2d(dst + F::kKvBytes + d * KT * 2, &mapV, &kv_full[stage], x + d, k0);
+      }
+      ++ls.kv_issued;
+      if (++ls.lj == it.n_tiles) {
+        ++ls.lk;
+        ls.lj = 0;
+      }
+    }
+  };
+  auto issue_q = [&](int k) {
+    const Item& it = item_at(k);
+    mbar_expect_tx(&q_full, F::kQBytes);
+#pragma unroll
+    for (int d = 0; d < DH; d += 64)
+      tma_load_2d(sQ + d * QT * 2, &mapQ, &q_full, it.h * DH + d, it.row0);
+    ++ls.q_issued;
+    ls.q_item = k;
+  };
+  // Q for the next item with key tiles within the decoded chunks
+  auto prefetch_q = [&](int k, int chunk_hi) {
+    if (k + 1 < min(cnt, (chunk_hi + 1) * CHUNK) && item_at(k + 1).n_tiles > 0) issue_q(k + 1);
+  };
+  // ---- MMAs (thread 0) ----
+  // S of K/V tile t (the first of its item: wait for Q too); false if a wait ran out
+  auto issue_s = [&](bool first, uint32_t t) -> bool {
+    if (first) {
+      if (!mbar_wait(&q_full, ls.q_done & 1)) return false;
+      ++ls.q_done;
+    }
+    if (!mbar_wait(&kv_full[t % KV_STAGES], (t / KV_STAGES) & 1)) return false;
+    ++ls.kv_done;
+    fence_after_sync();
+    const uint32_t q_addr = smem_u32(sQ);
+    const uint32_t k_addr = smem_u32(sKV + (t % KV_STAGES) * 2 * F::kKvBytes);
+#pragma unroll
+    for (int kk = 0; kk < DH / 16; ++kk)
+      mma_bf16(tmem + F::kColS, desc_kmajor_sw128(q_addr + kk / 4 * 64 * QT * 2 + kk % 4 * 32),
+               desc_kmajor_sw128(k_addr + kk / 4 * 64 * KT * 2 + kk % 4 * 32), IDESC_S, kk != 0);
+    mma_commit(&s_full);
+    ls.s_issued = t + 1;
+    return true;
+  };
+
+  // ---- the window of table biases: staged one tile ahead into win[g & 1] ----
+  float w0 = 0.f, w1 = 0.f;
+  auto win_load = [&](int h, int pos0, int entry) {  // this thread's two entries
+    if (REL == REL_WINDOW) {
+      const float* rel = p.rel_bias + (int64_t)h * (2 * (int64_t)p.rel_max + 1) + p.rel_max;
+      const int d = first_key(entry) - (pos0 + QT - 1) + tid;
+      w0 = rel[min(max(d, -p.rel_max), p.rel_max)];
+      if (tid < WIN - QT) w1 = rel[min(max(d + QT, -p.rel_max), p.rel_max)];
+    }
+  };
+  auto win_store = [&](uint32_t g) {
+    if (REL == REL_WINDOW) {
+      win[g & 1][tid] = bias_log2(w0);
+      if (tid < WIN - QT) win[g & 1][tid + QT] = bias_log2(w1);
+    }
+  };
+
+  const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+  const uint32_t tS = tmem + F::kColS + lane_off, tO = tmem + F::kColO + lane_off;
+  uint32_t g = 0;  // K/V tiles consumed (over items)
+  int fail = 0;    // a wait ran out (uniform within each warp)
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    int okw = 1;
+    if (lane == 0) okw = mbar_wait(bar, parity) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, okw, 0) != 0;
+  };
+  auto join = [&](int w) {  // after a section that lane 0 of warp w ran alone
+    if (warp == w) {
+      __syncwarp();
+      fail |= __shfl_sync(0xffffffffu, fail, 0);
+    }
+  };
+  if (REL == REL_WINDOW && cnt > 0) {
+    if (item_at(0).n_tiles > 0) {
+      win_load(item_at(0).h, item_at(0).pos0, item_at(0).first);
+      win_store(0);
+    }
+    __syncthreads();
+  }
+  // scores in units of log2: RAW scale2 s; CAP cap2 tanh(scale_y s)
+  const float scale2 = p.scale * kLog2e;
+  const float scale_y = CAP ? p.scale / p.cap : 0.f, cap2 = p.cap * kLog2e;
+
+  for (int k = 0; k < cnt; ++k) {
+    if (k > 0 && k % CHUNK == 0) {
+      if (__syncthreads_or(fail)) break;
+      decode_chunk(k / CHUNK + 1);
+      if (__syncthreads_or(fail)) break;
+    }
+    const int chunk_hi = k / CHUNK + 1;
+    const Item it = item_at(k);
+    const bool live = tid < it.rows;
+    const bool warp_live = warp * 32 < it.rows;
+    bf16* orow = p.O + (int64_t)(it.row0 + tid) * p.ldo + (int64_t)it.h * DH;
+    if (it.n_tiles == 0) {  // no row of the item sees a key
+      if (live)
+        for (int q = 0; q < DH / 8; ++q) reinterpret_cast<uint4*>(orow)[q] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    if (loader && !fail) {
+      if (ls.q_item != k) issue_q(k);
+      issue_kv(g, chunk_hi);
+    }
+    join(3);
+    // the row's intervals; rows past the item's end take the first row's
+    const int64_t rr = it.row0 + (live ? tid : 0);
+    const int4 ra = p.rows[2 * rr];
+    const int b1 = p.rows[2 * rr + 1].x;
+    const int pos = ra.x;
+    const float slope2 = SLOPE ? p.slopes[it.h] * kLog2e : 0.f;
+    const float* rel = REL == REL_DIRECT
+                           ? p.rel_bias + (int64_t)it.h * (2 * (int64_t)p.rel_max + 1) + p.rel_max
+                           : nullptr;
+    float m_ref = -INFINITY, l = 0.f;
+    int entry = it.first;
+    bool broke = false;
+    for (int j = 0; j < it.n_tiles; ++j, ++g) {
+      const int k0 = first_key(entry);
+      const bool full = entry < 0;
+      // the next tile of this CTA: its entry, and its window's values
+      const bool more = j + 1 < it.n_tiles;
+      if (more) entry = p.tiles[it.tile0 + j + 1];
+      const bool next = more || (k + 1 < cnt && item_at(k + 1).n_tiles > 0);
+      if (REL == REL_WINDOW && next) {
+        if (more) win_load(it.h, it.pos0, entry);
+        else win_load(item_at(k + 1).h, item_at(k + 1).pos0, item_at(k + 1).first);
+      }
+      if (leader && !fail && ls.s_issued <= g) {
+        if (!issue_s(j == 0, g)) {
+          record_err(10);
+          fail = 1;
+        }
+      }
+      join(0);
+      if (!fail && !warp_wait(&s_full, g & 1)) {
+        if (lane == 0) record_err(11);
+        fail = 1;
+      }
+      // Q is free once this item's last S is done: fetch the next item's
+      if (loader && !fail && !more) prefetch_q(k, chunk_hi);
+      join(3);
+      if (!fail && warp_live) {
+        fence_after_sync();
+        uint32_t s[KT];
+        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+        tmem_ld_wait();
+        if constexpr (!RAW) {
+          const float* wr = REL == REL_WINDOW ? &win[g & 1][QT - 1 - tid] : nullptr;
+          const int d0 = k0 - pos;
+          const float df = (float)d0;
+#pragma unroll
+          for (int c = 0; c < KT; c += 2) {
+            float b0 = 0.f, b1v = 0.f;
+            if (REL == REL_WINDOW) {
+              b0 = wr[c];
+              b1v = wr[c + 1];
+            } else if (REL == REL_DIRECT) {
+              b0 = bias_log2(rel[min(max(d0 + c, -p.rel_max), p.rel_max)]);
+              b1v = bias_log2(rel[min(max(d0 + c + 1, -p.rel_max), p.rel_max)]);
+            }
+            if (SLOPE) {
+              b0 = fmaf(-slope2, fabsf(df + (float)c), b0);
+              b1v = fmaf(-slope2, fabsf(df + (float)(c + 1)), b1v);
+            }
+            f32x2 x = pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            f32x2 f = splat2(scale2);
+            if (CAP) {
+              const float2 y = unpk2(mul2(x, splat2(scale_y)));
+              x = pk2(tanh_mufu(y.x), tanh_mufu(y.y));
+              f = splat2(cap2);
+            }
+            const float2 o = unpk2(fma2(x, f, pk2(b0, b1v)));
+            s[c] = __float_as_uint(o.x);
+            s[c + 1] = __float_as_uint(o.y);
+          }
+        }
+        if (!full) {
+          const uint64_t vis = bit_range(ra.y - k0, ra.z - k0) | bit_range(ra.w - k0, b1 - k0);
+          const uint32_t lo = (uint32_t)vis, hi = (uint32_t)(vis >> 32);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (!((lo >> c) & 1)) s[c] = __float_as_uint(-INFINITY);
+            if (!((hi >> c) & 1)) s[32 + c] = __float_as_uint(-INFINITY);
+          }
+        }
+        float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < KT; c += 8) {
+          a0 = max3(a0, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+          a1 = max3(a1, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+          a2 = max3(a2, __uint_as_float(s[c + 4]), __uint_as_float(s[c + 5]));
+          a3 = max3(a3, __uint_as_float(s[c + 6]), __uint_as_float(s[c + 7]));
+        }
+        float m_tile = max3(a0, a1, fmaxf(a2, a3));
+        if (RAW && m_tile != -INFINITY) m_tile *= scale2;
+        const bool first = m_ref == -INFINITY;
+        const bool grow = !first && m_tile > m_ref + kRescaleLog2;
+        const float m_new = (first || grow) ? m_tile : m_ref;
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float resc = grow ? ex2_approx(m_ref - m_new) : 1.f;
+        if (grow) l *= resc;
+        m_ref = m_new;
+        f32x2 acc0 = splat2(0.f), acc1 = splat2(0.f);
+        const f32x2 f = splat2(scale2), negm = splat2(-m_use);
+        uint32_t pk[KT / 2];
+#pragma unroll
+        for (int c = 0; c < KT; c += 2) {
+          f32x2 x = pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+          x = RAW ? fma2(x, f, negm) : add2(x, negm);
+          const float2 e = unpk2(x);
+          const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
+          if ((c >> 1) & 1) acc1 = add2(acc1, pk2(p0, p1));
+          else acc0 = add2(acc0, pk2(p0, p1));
+          const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+          pk[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        tmem_st32(tS, pk);
+        const float2 u0 = unpk2(acc0), u1 = unpk2(acc1);
+        l += (u0.x + u0.y) + (u1.x + u1.y);
+        if (__any_sync(0xffffffffu, grow) && j > 0) {
+          // O holds the earlier tiles against the old reference (their P V are done)
+#pragma unroll
+          for (int d = 0; d < DH; d += 32) {
+            uint32_t ov[32];
+            tmem_ld32(tO + d, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * resc);
+            tmem_st32(tO + d, ov);
+          }
+        }
+        tmem_st_wait();
+      }
+      if (next) win_store(g + 1);
+      fence_before_sync();
+      if (__syncthreads_or(fail)) {
+        broke = true;
+        break;
+      }
+      // O += P V, then the next S at once; the loader issues the loads that P V frees
+      if (leader) {
+        fence_after_sync();
+        const uint32_t v_addr = smem_u32(sKV + (g % KV_STAGES) * 2 * F::kKvBytes + F::kKvBytes);
+#pragma unroll
+        for (int d = 0; d < DH; d += 64)
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk)
+            mma_bf16_ts(tmem + F::kColO + d, tmem + F::kColS + kk * 8,
+                        desc_mnmajor_sw128(v_addr + d * KT * 2 + kk * 16 * 128), IDESC_O,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&pv_done);
+        if (!mbar_wait(&pv_done, g & 1)) {
+          record_err(12);
+          fail = 1;
+        } else {
+          bool go = kv_out() > g + 1 && (more || q_out_item() > k);
+          if (go && !more) go = mbar_test(&q_full, ls.q_done & 1);
+          if (go && !issue_s(!more, g + 1)) {
+            record_err(10);
+            fail = 1;
+          }
+        }
+      }
+      join(0);
+      if (loader) {
+        if (!mbar_wait(&pv_done, g & 1)) {
+          record_err(12);
+          fail = 1;
+        } else {
+          issue_kv(g + 1, chunk_hi);
+        }
+      }
+      join(3);
+    }
+    if (broke) break;
+    if (!fail && !warp_wait(&pv_done, (g - 1) & 1)) {
+      if (lane == 0) record_err(13);
+      fail = 1;
+    }
+    if (fail) continue;  // carried to the next block-wide barrier
+    if (!warp_live) continue;
+    fence_after_sync();
+    // no visible key, or only scores of -inf: 0 (a NaN in l stays one)
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float odd = 0.f;  // stays 0 while every output is finite
+#pragma unroll
+    for (int d = 0; d < DH; d += 32) {
+      uint32_t ov[32];
+      tmem_ld32(tO + d, ov);
+      tmem_ld_wait();
+      uint32_t w[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float a = __uint_as_float(ov[2 * e]) * inv, b = __uint_as_float(ov[2 * e + 1]) * inv;
+        odd = fmaf(a, 0.f, odd);
+        odd = fmaf(b, 0.f, odd);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      if (live) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          reinterpret_cast<uint4*>(orow + d)[q] =
+              make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      }
+    }
+    fence_before_sync();
+    unsigned again = __ballot_sync(0xffffffffu, odd != 0.f && live);
+    while (again) {
+      const int r = __ffs(again) - 1;
+      again &= again - 1;
+      const int row = it.row0 + warp * 32 + r;
+      float o[4];
+      attn_masked_row(p, row, it.h, lane, o);
+      bf16* out = p.O + (int64_t)row * p.ldo + (int64_t)it.h * DH;
+#pragma unroll
+      for (int c = 0; c < DH / 32; ++c) out[lane + 32 * c] = __float2bfloat16(o[c]);
+    }
+  }
+
+  // every issued copy has landed and every MMA is done before TMEM and shared
+  // memory are released
+  __syncthreads();
+  if (leader) {
+    if (ls.q_issued > ls.q_done && !mbar_wait(&q_full, ls.q_done & 1)) record_err(14);
+    for (uint32_t t = ls.kv_done; t < ls.kv_issued; ++t)
+      if (!mbar_wait(&kv_full[t % KV_STAGES], (t / KV_STAGES) & 1)) record_err(15);
+    mma_commit(&drain);
+    if (!mbar_wait(&drain, 0)) record_err(16);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    fence_after_sync();
+    tmem_dealloc(tmem, F::kTmemCols);
+  }
+}
+
+template <int DH, bool RAW, bool CAP, int REL, bool SLOPE>
+cudaError_t launch(const AttnMasked& p, cudaStream_t st) {
+  using F = Shape<DH>;
+  static std::atomic<uint64_t> attr_done{0};  // per device ordinal
+  auto kernel = attn_masked_tc_kernel<DH, RAW, CAP, REL, SLOPE>;
+  if (cudaError_t rc = ensure_smem_attr(kernel, F::kSmem, attr_done)) return rc;
+  CUtensorMap mq, mk, mv;
+  if (!make_map_bf16(&mq, p.q, (uint64_t)p.H * DH, p.n_rows, (uint64_t)p.ldq * 2, 64, QT) ||
+      !make_map_bf16(&mk, p.k, (uint64_t)p.Hkv * DH, p.n_keys, (uint64_t)p.ldk * 2, 64, KT) ||
+      !make_map_bf16(&mv, p.v, (uint64_t)p.Hkv * DH, p.n_keys, (uint64_t)p.ldv * 2, 64, KT))
+    return cudaErrorInvalidValue;
+  const int64_t work = (int64_t)p.n_items * p.H;
+  if (work > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const int grid = (int)std::min<int64_t>(work, (int64_t)F::kCtas * sm_count());
+  kernel<<<grid, kThreads, F::kSmem, st>>>(mq, mk, mv, p, (int)work);
+  return cudaGetLastError();
+}
+
+template <int DH>
+cudaError_t dispatch(const AttnMasked& p, cudaStream_t st) {
+  // consecutive query rows read table biases through the staged window
+  const int rel = !p.rel_bias ? REL_NONE : p.rows_consecutive ? REL_WINDOW : REL_DIRECT;
+  const bool cap = p.cap > 0.f, slope = p.slopes != nullptr;
+  if (rel == REL_NONE) {
+    // RAW scales after the mask, so it needs a scale that keeps -inf
+    if (!cap && !slope && p.scale > 1e-30f) return launch<DH, true, false, REL_NONE, false>(p, st);
+    if (!slope) return cap ? launch<DH, false, true, REL_NONE, false>(p, st)
+                           : launch<DH, false, false, REL_NONE, false>(p, st);
+    return cap ? launch<DH, false, true, REL_NONE, true>(p, st)
+               : launch<DH, false, false, REL_NONE, true>(p, st);
+  }
+  if (rel == REL_WINDOW) {
+    if (!slope) return cap ? launch<DH, false, true, REL_WINDOW, false>(p, st)
+                           : launch<DH, false, false, REL_WINDOW, false>(p, st);
+    return cap ? launch<DH, false, true, REL_WINDOW, true>(p, st)
+               : launch<DH, false, false, REL_WINDOW, true>(p, st);
+  }
+  if (!slope) return cap ? launch<DH, false, true, REL_DIRECT, false>(p, st)
+                         : launch<DH, false, false, REL_DIRECT, false>(p, st);
+  return cap ? launch<DH, false, true, REL_DIRECT, true>(p, st)
+             : launch<DH, false, false, REL_DIRECT, true>(p, st);
+}
+
+}  // namespace
+
+// head_dim 64 or 128 with 16-byte rows and addresses; the rest runs on CUDA cores.
+bool attn_masked_tc_supported(const AttnMasked& p) {
+  auto on = [](const void* q) { return !(reinterpret_cast<uintptr_t>(q) & 15); };
+  return (p.Dh == 64 || p.Dh == 128) && p.n_keys > 0 && p.ldq % 8 == 0 && p.ldk % 8 == 0 &&
+         p.ldv % 8 == 0 && p.ldo % 8 == 0 && on(p.q) && on(p.k) && on(p.v) && on(p.O) &&
+         on(p.rows);
+}
+
+cudaError_t attn_masked_tc(const AttnMasked& p, cudaStream_t st) {
+  return p.Dh == 64 ? dispatch<64>(p, st) : dispatch<128>(p, st);
+}
+
+cudaError_t attn_masked_take_status(int* code) {
+  int v = 0;
+  cudaError_t rc = cudaMemcpyFromSymbol(&v, g_attn_masked_err, sizeof(int));
+  if (rc == cudaSuccess && v != 0) {
+    const int zero = 0;
+    rc = cudaMemcpyToSymbol(g_attn_masked_err, &zero, sizeof(int));
+  }
+  *code = v;
+  return rc;
+}
+
+}  // namespace sjb

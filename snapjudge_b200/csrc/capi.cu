@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "../../include/snapjudge_b200.h"
+#include "attn_masked.cuh"
 #include "common.cuh"
 #include "gemm_lora.cuh"
 #include "kernels.h"
@@ -184,6 +185,9 @@ int sj_check_device_errors(void* stream) {
   int a = 0, g = 0, sc = 0, al = 0, gl = 0;
   if ((rc = sjb::attn_tc_take_status(&a)) != cudaSuccess) return launched(rc, "attention status");
   if ((rc = sjb::attn_long_take_status(&al)) != cudaSuccess)
+    return launched(rc, "attention status");
+  if (!a) a = al;
+  if ((rc = sjb::attn_masked_take_status(&al)) != cudaSuccess)
     return launched(rc, "attention status");
   if (!a) a = al;
   if ((rc = sjb::gemm_tc_take_status(&g)) != cudaSuccess) return launched(rc, "GEMM status");
