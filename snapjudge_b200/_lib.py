@@ -122,17 +122,16 @@ def lib() -> C.CDLL:
         L.sj_test_attn_wait_timeout.restype = None
         L.sj_quant_e4m3.argtypes = [_P, C.c_int64, _I, _P, _P, _P]
         L.sj_gemm_e4m3.argtypes = [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]
-        L.sj_attn_plan.argtypes = [C.POINTER(AttnPlanArgs), _P, _L, C.POINTER(AttnPlanInfo)]
-        L.sj_attn_masked_workspace.argtypes = [C.POINTER(AttnPlanInfo), _I, _I, _I]
+        # structures go by address (a ctypes structure by reference, or its bytes)
+        L.sj_attn_plan.argtypes = [_P, _P, _L, _P]
+        L.sj_attn_masked_workspace.argtypes = [_P, _I, _I, _I]
         L.sj_attn_masked_workspace.restype = _L
-        L.sj_attn_masked.argtypes = [C.POINTER(AttnMaskedArgs), C.POINTER(AttnPlanInfo), _P, _P,
-                                     _L, _P]
-        L.sj_lora_plan.argtypes = [_P, _I, _P, _I, _I, _P, _L, C.POINTER(LoraPlanInfo)]
-        L.sj_gemm_lora_workspace.argtypes = [C.POINTER(LoraPlanInfo), _I, _I]
+        L.sj_attn_masked.argtypes = [_P, _P, _P, _P, _L, _P]
+        L.sj_lora_plan.argtypes = [_P, _I, _P, _I, _I, _P, _L, _P]
+        L.sj_gemm_lora_workspace.argtypes = [_P, _I, _I]
         L.sj_gemm_lora_workspace.restype = _L
-        L.sj_gemm_lora.argtypes = [C.POINTER(GemmLoraArgs), C.POINTER(LoraPlanInfo), _P, _P, _L,
-                                   _P]
-        L.sj_norm_block.argtypes = [C.POINTER(NormBlockArgs), _P]
+        L.sj_gemm_lora.argtypes = [_P, _P, _P, _P, _L, _P]
+        L.sj_norm_block.argtypes = [_P, _P]
         L.sj_fast_create.argtypes = [C.POINTER(FastConfig), C.POINTER(_P)]
         L.sj_fast_set_tensor.argtypes = [_P, C.c_char_p, _P, C.POINTER(C.c_int64), _I]
         L.sj_fast_set_heads.argtypes = [_P, _I, C.POINTER(_I), C.POINTER(_I)]

@@ -12,7 +12,13 @@
 //   row sees whole skip this); p = 2^(x - m), m the row's reference maximum;
 //   P (bf16 pairs) over S in TMEM; O += P V.
 // Several such CTAs share an SM (4 at head_dim 64, 2 at 128), so that one's
-// softmax runs beside another's MMAs.
+// softmax runs beside another's MMAs.  What bounds it is the softmax's
+// instructions (8 to 15 for each score; issue slots about half used).  Measured
+// on 256 x (state + six questions), 12 heads, and on 16 x 2048 with a cap and
+// slopes, 16 heads (us): this form 354 and 762; three chains of 128 threads in
+// one CTA with P in columns of its own, so that MMAs overlap the softmax, 554 and
+// 1,341; two chains with warps of their own for loads, MMAs and work lists, 748
+// and 1,218: fewer softmax warps cost more than the overlap gains.
 // The reference maximum moves only when a tile's maximum exceeds it by 2^8; the
 // row's O in TMEM and its sum are then rescaled.  Sums and O are fp32; P is
 // rounded to bf16 because V is bf16 and the MMA takes one type.
@@ -24,6 +30,8 @@
 // keys alone (attn_masked_row).
 // Waits are bounded and failures carried to the next block-wide barrier, as in
 // attn_tc.cu.
+#include <string.h>
+
 #include <algorithm>
 #include <atomic>
 
@@ -43,10 +51,20 @@ using namespace tc;
 constexpr int QT = 128, KT = 64;
 constexpr int kThreads = 128;
 constexpr int KV_STAGES = 2;
+// Of every 8 column pairs this many are exponentiated on the FMA pipe (ex2_poly):
+// 1 without a cap (0: +4 %, 2: +7 %); the cap's polynomial leaves no room for it.
+template <bool CAP>
+constexpr int poly_pairs() { return CAP ? 0 : 1; }
 constexpr int CHUNK = 32;  // work items decoded at a time
 constexpr float kRescaleLog2 = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int WIN = QT + KT;  // staged distances (191 used)
+// Staged distances: 191 used.  Two copies, the second one entry ahead, so that
+// a row's pair of columns is one aligned 8-byte load whatever the row; the
+// second starts 16 banks on, so that a half-warp's loads do not collide.
+constexpr int WIN = QT + KT, WIN_COPY = 208;
+// tanh(y) for |y| <= 1 as an odd polynomial, y (c0 + u (c1 + ...)), u = y^2:
+// minimax fit on Chebyshev nodes, relative error <= 8e-6
+constexpr float kTanh[5] = {0.9999939f, -0.33300743f, 0.13050084f, -0.04502869f, 0.00914157f};
 
 enum Rel { REL_NONE = 0, REL_WINDOW = 1, REL_DIRECT = 2 };
 
@@ -90,6 +108,151 @@ __device__ __forceinline__ uint64_t bit_range(int a, int b) {
   return (~0ull >> (64 - (b - a))) << a;
 }
 
+// Scores of a row in place: s <- cap2 tanh(sy s) or scale2 s, plus bias, in units
+// of log2.  A step whose cap arguments stay within 1 in the whole warp takes the
+// polynomial (FMA pipe); others the tanh unit, which shares the MUFU with the
+// exponentials.
+struct Score {  // constants of a call; pairs hold a value twice
+  f32x2 scale2;  // no cap: scale log2(e)
+  f32x2 c[5];    // cap: cap2 sy^(2i+1) kTanh[i]
+  f32x2 sy;      // cap: scale / cap
+  f32x2 cap2;    // cap: cap log2(e)
+  float lim;     // cap: |s| up to which |sy s| <= 1 (-1: never)
+  float scale2f;
+};
+f32x2 twice(float v) {
+  uint32_t b;
+  memcpy(&b, &v, 4);
+  return ((f32x2)b << 32) | b;
+}
+Score make_score(const AttnMasked& p) {
+  Score k{};
+  k.scale2f = p.scale * kLog2e;
+  k.scale2 = twice(k.scale2f);
+  if (p.cap > 0.f) {
+    const float sy = p.scale / p.cap, cap2 = p.cap * kLog2e, u = sy * sy;
+    k.sy = twice(sy);
+    k.cap2 = twice(cap2);
+    // the coefficients' powers of sy have to stay well inside the type's range
+    k.lim = u > 1e-7f && u < 1e7f ? 1.f / fabsf(sy) : -1.f;
+    float f = cap2 * sy;
+    for (int i = 0; i < 5; ++i, f *= u) k.c[i] = twice(kTanh[i] * f);
+  }
+  return k;
+}
+// The passes below run straight through all of a tile's columns and branch, for
+// the whole warp, between passes only: with branches for each 16 or 32 columns
+// the same work took 1.1 to 1.4 times as long.
+__device__ __forceinline__ void tanh_pair(uint32_t* s, f32x2 x, const Score& k) {
+  const float2 y = unpk2(mul2(x, k.sy));
+  const float2 o = unpk2(mul2(pk2(tanh_mufu(y.x), tanh_mufu(y.y)), k.cap2));
+  s[0] = __float_as_uint(o.x);
+  s[1] = __float_as_uint(o.y);
+}
+// Half of the pairs take the polynomial and half the tanh unit: all on the one
+// keeps the FMA pipe, all on the other the MUFU, busier than the rest (16 x 2048
+// with a cap, 16 heads: 715 and 733 us against 676).
+template <int N>
+__device__ __forceinline__ void cap_scores(uint32_t (&s)[N], const Score& k) {
+  float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+  for (int c = 0; c < N; c += 4) {
+    a0 = max3(a0, fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
+    a1 = max3(a1, fabsf(__uint_as_float(s[c + 2])), fabsf(__uint_as_float(s[c + 3])));
+  }
+  if (__all_sync(0xffffffffu, fmaxf(a0, a1) <= k.lim)) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const f32x2 x = pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+      if ((c >> 1) & 1) {
+        tanh_pair(s + c, x, k);
+        continue;
+      }
+      const f32x2 u = mul2(x, x);
+      f32x2 q = fma2(u, k.c[4], k.c[3]);
+      q = fma2(u, q, k.c[2]);
+      q = fma2(u, q, k.c[1]);
+      q = fma2(u, q, k.c[0]);
+      const float2 o = unpk2(mul2(x, q));
+      s[c] = __float_as_uint(o.x);
+      s[c + 1] = __float_as_uint(o.y);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      tanh_pair(s + c, pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), k);
+    }
+  }
+}
+// s[c] <- s[c] (or, without a cap, scale2 s[c]) + the bias of a tile's 64 columns,
+// at distances d + c.  LIN: the warp's pairs lie on one side (kk d is their slope
+// bias), else it is kk |d|.
+template <bool CAP, int REL, bool SLOPE, bool LIN>
+__device__ __forceinline__ void bias_tile(uint32_t* s, const Score& k, const float* wr,
+                                          const AttnMasked& p, const float* rel, int d, float kk) {
+  const float df = (float)d;
+  f32x2 b2 = splat2(0.f), step2 = splat2(0.f);
+  if (SLOPE && LIN) {
+    b2 = pk2(kk * df, fmaf(kk, df, kk));
+    step2 = splat2(2.f * kk);
+  }
+#pragma unroll
+  for (int c = 0; c < KT; c += 2) {
+    f32x2 b = splat2(0.f);
+    if (REL == REL_WINDOW) {
+      const float2 v = *reinterpret_cast<const float2*>(wr + c);
+      b = pk2(v.x, v.y);
+    } else if (REL == REL_DIRECT) {
+      b = pk2(bias_log2(rel[min(max(d + c, -p.rel_max), p.rel_max)]),
+              bias_log2(rel[min(max(d + c + 1, -p.rel_max), p.rel_max)]));
+    }
+    if (SLOPE) {
+      if (LIN) {
+        b = REL == REL_NONE ? b2 : add2(b, b2);
+        b2 = add2(b2, step2);
+      } else {
+        const float2 v = unpk2(b);
+        b = pk2(fmaf(kk, fabsf(df + (float)c), v.x), fmaf(kk, fabsf(df + (float)(c + 1)), v.y));
+      }
+    }
+    const f32x2 x = pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+    const float2 o = unpk2(CAP ? add2(x, b) : fma2(x, k.scale2, b));
+    s[c] = __float_as_uint(o.x);
+    s[c + 1] = __float_as_uint(o.y);
+  }
+}
+template <int N>
+__device__ __forceinline__ float max_scores(const uint32_t (&r)[N]) {
+  float a = -INFINITY, b = -INFINITY, c = -INFINITY, d = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; i += 8) {
+    a = max3(a, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+    b = max3(b, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+    c = max3(c, __uint_as_float(r[i + 4]), __uint_as_float(r[i + 5]));
+    d = max3(d, __uint_as_float(r[i + 6]), __uint_as_float(r[i + 7]));
+  }
+  return max3(a, b, fmaxf(c, d));
+}
+
+// 2^x for a pair on the FMA and ALU pipes: x = n + f with n = rint(x) (adding
+// 1.5 2^23 leaves it in the low mantissa bits), 2^f by a cubic fitted by least
+// squares on Chebyshev nodes of [-0.5, 0.5] (relative error <= 7.5e-5, far below
+// the rounding of P), 2^n into the exponent.  Below -125 the result is 2^-125,
+// which vanishes beside the row's maximum; -inf (a masked key) gives 0.
+__device__ __forceinline__ f32x2 ex2_poly(f32x2 x) {
+  const float2 v = unpk2(x);
+  const f32x2 xv = pk2(fmaxf(v.x, -125.f), fmaxf(v.y, -125.f));
+  const f32x2 t = add2(xv, splat2(12582912.f));
+  const f32x2 f = fma2(add2(t, splat2(-12582912.f)), splat2(-1.f), xv);
+  f32x2 q = fma2(splat2(0.0551716238f), f, splat2(0.242611125f));
+  q = fma2(q, f, splat2(0.693260968f));
+  q = fma2(q, f, splat2(0.999928057f));
+  const float2 qf = unpk2(q), tf = unpk2(t);
+  const float a = __uint_as_float(__float_as_uint(qf.x) + (__float_as_uint(tf.x) << 23));
+  const float b = __uint_as_float(__float_as_uint(qf.y) + (__float_as_uint(tf.y) << 23));
+  return pk2(v.x == -INFINITY ? 0.f : a, v.y == -INFINITY ? 0.f : b);
+}
+
 struct __align__(16) Item {
   int row0, rows, tile0, n_tiles;
   int h, first, pos0, pad;  // head, first key-tile entry, position of the first row
@@ -100,7 +263,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
     attn_masked_tc_kernel(const __grid_constant__ CUtensorMap mapQ,
                           const __grid_constant__ CUtensorMap mapK,
                           const __grid_constant__ CUtensorMap mapV,
-                          const __grid_constant__ AttnMasked p, int n_work) {
+                          const __grid_constant__ AttnMasked p, const __grid_constant__ Score sc,
+                          int n_work) {
   using F = Shape<DH>;
   constexpr uint32_t IDESC_S = idesc_bf16(QT, KT, false, false);
   constexpr uint32_t IDESC_O = idesc_bf16(QT, 64, false, true);
@@ -108,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
   __shared__ uint64_t q_full, kv_full[KV_STAGES], s_full, pv_done, drain;
   __shared__ Item items[2][CHUNK];  // this CTA's work items, chunk c in items[c & 1]
   __shared__ uint32_t tmem_sh;
-  __shared__ float win[REL == REL_WINDOW ? 2 : 1][REL == REL_WINDOW ? WIN : 1];
+  __shared__ __align__(16) float win[REL == REL_WINDOW ? 2 : 1][REL == REL_WINDOW ? 2 * WIN_COPY : 4];
   __shared__ struct {
     int lk, lj;          // loader: next K/V tile to load: item lk, tile lj
     uint32_t kv_issued, q_issued;
@@ -170,6 +334,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
   auto q_out_item = [&]() { return *reinterpret_cast<volatile int*>(&ls.q_item); };
 
   // ---- loads (thread 96) ----
+  int entry_ahead = 0;  // of tile lj > 0 of item lk: read when its predecessor was issued
   auto issue_kv = [&](uint32_t released, int chunk_hi) {
     const int k_end = min(cnt, (chunk_hi + 1) * CHUNK);
     while (ls.kv_issued < released + KV_STAGES && ls.lk < k_end) {
@@ -180,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
         continue;
       }
       const int stage = ls.kv_issued % KV_STAGES;
-      const int k0 = first_key(ls.lj == 0 ? it.first : p.tiles[it.tile0 + ls.lj]);
+      const int k0 = first_key(ls.lj == 0 ? it.first : entry_ahead);
       const int x = it.h / group * DH;
       uint8_t* dst = sKV + stage * 2 * F::kKvBytes;
       mbar_expect_tx(&kv_full[stage], 2 * F::kKvBytes);
@@ -193,6 +358,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
       if (++ls.lj == it.n_tiles) {
         ++ls.lk;
         ls.lj = 0;
+      } else {
+        entry_ahead = p.tiles[it.tile0 + ls.lj];
       }
     }
   };
@@ -242,8 +409,14 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
   };
   auto win_store = [&](uint32_t g) {
     if (REL == REL_WINDOW) {
-      win[g & 1][tid] = bias_log2(w0);
-      if (tid < WIN - QT) win[g & 1][tid + QT] = bias_log2(w1);
+      float* w = win[g & 1];
+      const float v0 = bias_log2(w0), v1 = bias_log2(w1);
+      w[tid] = v0;
+      if (tid > 0) w[WIN_COPY + tid - 1] = v0;
+      if (tid < WIN - QT) {
+        w[tid + QT] = v1;
+        w[WIN_COPY + tid + QT - 1] = v1;
+      }
     }
   };
 
@@ -269,10 +442,6 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
     }
     __syncthreads();
   }
-  // scores in units of log2: RAW scale2 s; CAP cap2 tanh(scale_y s)
-  const float scale2 = p.scale * kLog2e;
-  const float scale_y = CAP ? p.scale / p.cap : 0.f, cap2 = p.cap * kLog2e;
-
   for (int k = 0; k < cnt; ++k) {
     if (k > 0 && k % CHUNK == 0) {
       if (__syncthreads_or(fail)) break;
@@ -331,85 +500,82 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
       // Q is free once this item's last S is done: fetch the next item's
       if (loader && !fail && !more) prefetch_q(k, chunk_hi);
       join(3);
-      if (!fail && warp_live) {
+      if (!more && k + 1 < cnt) {  // the next item's row records
+        const Item& nx = item_at(k + 1);
+        if (tid < nx.rows)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(p.rows + 2 * (int64_t)(nx.row0 + tid)));
+      }
+      uint64_t bits = ~0ull;
+      if (!full) bits = bit_range(ra.y - k0, ra.z - k0) | bit_range(ra.w - k0, b1 - k0);
+      const bool see = full || __any_sync(0xffffffffu, bits != 0);
+      if (!fail && warp_live && !see) {  // the warp sees nothing of the tile
         fence_after_sync();
-        uint32_t s[KT];
+        uint32_t zero[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) zero[c] = 0u;
+        tmem_st32(tS, zero);
+        tmem_st_wait();
+      } else if (!fail && warp_live) {
+        fence_after_sync();
+        uint32_t s[KT];  // scores, then P as bf16 pairs in the first half
         tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
         tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
         tmem_ld_wait();
-        if constexpr (!RAW) {
-          const float* wr = REL == REL_WINDOW ? &win[g & 1][QT - 1 - tid] : nullptr;
+        if constexpr (CAP) cap_scores(s, sc);
+        if constexpr (!RAW && (!CAP || REL != REL_NONE || SLOPE)) {
           const int d0 = k0 - pos;
-          const float df = (float)d0;
+          const int w_at = QT - 1 - tid;
+          const float* wr =
+              REL == REL_WINDOW ? &win[g & 1][w_at & 1 ? WIN_COPY + w_at - 1 : w_at] : nullptr;
+          // all of the warp's pairs on one side: the slope bias is linear
+          const bool up = !SLOPE || __all_sync(0xffffffffu, d0 >= 0);
+          if (!SLOPE || up || __all_sync(0xffffffffu, d0 <= 1 - KT))
+            bias_tile<CAP, REL, SLOPE, true>(s, sc, wr, p, rel, d0, up ? -slope2 : slope2);
+          else
+            bias_tile<CAP, REL, SLOPE, false>(s, sc, wr, p, rel, d0, -slope2);
+        }
+        if (!full) {  // mask, unless the warp sees the whole tile
+          const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+          if (!__all_sync(0xffffffffu, lo == ~0u)) {
 #pragma unroll
-          for (int c = 0; c < KT; c += 2) {
-            float b0 = 0.f, b1v = 0.f;
-            if (REL == REL_WINDOW) {
-              b0 = wr[c];
-              b1v = wr[c + 1];
-            } else if (REL == REL_DIRECT) {
-              b0 = bias_log2(rel[min(max(d0 + c, -p.rel_max), p.rel_max)]);
-              b1v = bias_log2(rel[min(max(d0 + c + 1, -p.rel_max), p.rel_max)]);
-            }
-            if (SLOPE) {
-              b0 = fmaf(-slope2, fabsf(df + (float)c), b0);
-              b1v = fmaf(-slope2, fabsf(df + (float)(c + 1)), b1v);
-            }
-            f32x2 x = pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-            f32x2 f = splat2(scale2);
-            if (CAP) {
-              const float2 y = unpk2(mul2(x, splat2(scale_y)));
-              x = pk2(tanh_mufu(y.x), tanh_mufu(y.y));
-              f = splat2(cap2);
-            }
-            const float2 o = unpk2(fma2(x, f, pk2(b0, b1v)));
-            s[c] = __float_as_uint(o.x);
-            s[c + 1] = __float_as_uint(o.y);
+            for (int c = 0; c < 32; ++c)
+              if (!((lo >> c) & 1)) s[c] = __float_as_uint(-INFINITY);
+          }
+          if (!__all_sync(0xffffffffu, hi == ~0u)) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!((hi >> c) & 1)) s[32 + c] = __float_as_uint(-INFINITY);
           }
         }
-        if (!full) {
-          const uint64_t vis = bit_range(ra.y - k0, ra.z - k0) | bit_range(ra.w - k0, b1 - k0);
-          const uint32_t lo = (uint32_t)vis, hi = (uint32_t)(vis >> 32);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (!((lo >> c) & 1)) s[c] = __float_as_uint(-INFINITY);
-            if (!((hi >> c) & 1)) s[32 + c] = __float_as_uint(-INFINITY);
-          }
-        }
-        float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < KT; c += 8) {
-          a0 = max3(a0, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-          a1 = max3(a1, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
-          a2 = max3(a2, __uint_as_float(s[c + 4]), __uint_as_float(s[c + 5]));
-          a3 = max3(a3, __uint_as_float(s[c + 6]), __uint_as_float(s[c + 7]));
-        }
-        float m_tile = max3(a0, a1, fmaxf(a2, a3));
-        if (RAW && m_tile != -INFINITY) m_tile *= scale2;
+        float m_tile = max_scores(s);
+        if (RAW && m_tile != -INFINITY) m_tile *= sc.scale2f;
         const bool first = m_ref == -INFINITY;
         const bool grow = !first && m_tile > m_ref + kRescaleLog2;
         const float m_new = (first || grow) ? m_tile : m_ref;
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
         const float resc = grow ? ex2_approx(m_ref - m_new) : 1.f;
-        if (grow) l *= resc;
+        l *= resc;
         m_ref = m_new;
+        const f32x2 negm = splat2(m_new == -INFINITY ? 0.f : -m_new);
         f32x2 acc0 = splat2(0.f), acc1 = splat2(0.f);
-        const f32x2 f = splat2(scale2), negm = splat2(-m_use);
-        uint32_t pk[KT / 2];
 #pragma unroll
         for (int c = 0; c < KT; c += 2) {
           f32x2 x = pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-          x = RAW ? fma2(x, f, negm) : add2(x, negm);
-          const float2 e = unpk2(x);
-          const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
-          if ((c >> 1) & 1) acc1 = add2(acc1, pk2(p0, p1));
-          else acc0 = add2(acc0, pk2(p0, p1));
-          const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-          pk[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+          x = RAW ? fma2(x, sc.scale2, negm) : add2(x, negm);
+          float2 pr;
+          if (((c >> 1) & 7) >= 8 - poly_pairs<CAP>()) {
+            pr = unpk2(ex2_poly(x));
+          } else {
+            const float2 v = unpk2(x);
+            pr = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+          }
+          if ((c >> 1) & 1) acc1 = add2(acc1, pk2(pr.x, pr.y));
+          else acc0 = add2(acc0, pk2(pr.x, pr.y));
+          const __nv_bfloat162 hb = __floats2bfloat162_rn(pr.x, pr.y);
+          s[c >> 1] = *reinterpret_cast<const uint32_t*>(&hb);
         }
-        tmem_st32(tS, pk);
         const float2 u0 = unpk2(acc0), u1 = unpk2(acc1);
         l += (u0.x + u0.y) + (u1.x + u1.y);
+        tmem_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
         if (__any_sync(0xffffffffu, grow) && j > 0) {
           // O holds the earlier tiles against the old reference (their P V are done)
 #pragma unroll
@@ -543,7 +709,7 @@ cudaError_t launch(const AttnMasked& p, cudaStream_t st) {
   const int64_t work = (int64_t)p.n_items * p.H;
   if (work > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const int grid = (int)std::min<int64_t>(work, (int64_t)F::kCtas * sm_count());
-  kernel<<<grid, kThreads, F::kSmem, st>>>(mq, mk, mv, p, (int)work);
+  kernel<<<grid, kThreads, F::kSmem, st>>>(mq, mk, mv, p, make_score(p), (int)work);
   return cudaGetLastError();
 }
 

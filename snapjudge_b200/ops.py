@@ -15,6 +15,7 @@ may be used on any stream.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -146,24 +147,54 @@ def _plan_on_device(buf, device):
 
 
 def _at(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _rows(t, name, dtype):
-    """A CUDA tensor whose last dimension is contiguous; returns its row pitch in elements."""
-    if not (t.is_cuda and t.dtype == dtype and t.dim() == 2):
-        raise ValueError(f"{name} must be a 2-D CUDA {dtype} tensor")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+def _here(t, name):
+    """t's CUDA device, which has to be the current one."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError(f"{name} must be a CUDA tensor on the current device")
+    return dev
+
+
+def _rows(t, name, dtype, dev):
+    """A 2-D tensor whose last dimension is contiguous; returns its row pitch in elements."""
+    if t.dtype is not dtype or t.dim() != 2 or t.get_device() != dev:
+        raise ValueError(f"{name} must be a 2-D {dtype} tensor on cuda:{dev}")
+    n, d = t.shape
+    ld, step = t.stride()
+    if step != 1 and d > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return ld if n > 1 else d
 
 
-def _vec(t, name, n):
-    """A contiguous CUDA fp32 tensor of shape n (or None)."""
-    if t is not None:
-        _need(t, torch.float32, name)
-        if tuple(t.shape) != n:
-            raise ValueError(f"{name} must have shape {n}, not {tuple(t.shape)}")
+def _vec(t, name, shape, dev, dtype=torch.float32):
+    """A contiguous tensor of that shape, or None; returns its address."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on "
+                         f"cuda:{dev}")
+    return t.data_ptr()
+
+
+# the current stream's handle without a Stream object around it (1.3 us less a call)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _packer(cls):
+    """A function that lays out a ctypes structure's fields as its bytes (an
+    order of magnitude faster than filling the structure)."""
+    code = {C.c_void_p: "P", C.c_int: "i", C.c_int32: "i", C.c_int64: "q", C.c_float: "f"}
+    fmt = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
+    assert fmt.size <= C.sizeof(cls) < fmt.size + 8
+    return struct.Struct(fmt.format + "0q").pack
+
+
+_attn_masked_args = _packer(_lib.AttnMaskedArgs)
+_gemm_lora_args = _packer(_lib.GemmLoraArgs)
+_norm_block_args = _packer(_lib.NormBlockArgs)
 
 
 class AttnPlan:
@@ -200,18 +231,22 @@ class AttnPlan:
         check(L.sj_attn_plan(C.byref(args), None, 0, C.byref(self.info)))
         buf = np.empty(max(1, self.info.plan_len), np.int32)
         check(L.sj_attn_plan(C.byref(args), buf.ctypes.data, len(buf), C.byref(self.info)))
+        self.info_ref = C.byref(self.info)
         self.n_rows, self.n_keys = self.info.n_rows, self.info.n_keys
         self.data = _plan_on_device(buf, device)
+        self.device = self.data.get_device()
+        self.workspace = {}  # bytes that a call needs, by head shape
 
 
-def _heads(t, name):
+def _heads(t, name, dev):
     """[rows, heads, Dh] bf16 with contiguous rows of heads; returns its row pitch."""
-    if not (t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 3):
-        raise ValueError(f"{name} must be a [rows, heads, head_dim] CUDA bfloat16 tensor")
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.get_device() != dev:
+        raise ValueError(f"{name} must be a [rows, heads, head_dim] bfloat16 tensor on cuda:{dev}")
     n, H, Dh = t.shape
-    if (Dh > 1 and t.stride(2) != 1) or (H > 1 and t.stride(1) != Dh):
+    ld, lh, step = t.stride()
+    if (step != 1 and Dh > 1) or (lh != Dh and H > 1):
         raise ValueError(f"{name}: a row's heads must be contiguous")
-    return t.stride(0) if n > 1 else H * Dh
+    return ld if n > 1 else H * Dh
 
 
 def attn_masked(q, k, v, plan, *, scale=None, softcap=0.0, rel_bias=None, slopes=None):
@@ -223,31 +258,36 @@ def attn_masked(q, k, v, plan, *, scale=None, softcap=0.0, rel_bias=None, slopes
     ``softcap tanh(x / softcap)`` when softcap > 0, plus ``rel_bias[h,
     clamp(d, -R, R) + R]`` (fp32 [H, 2R + 1]), minus ``slopes[h] |d|`` (fp32
     [H]).  A row that sees no key gives 0."""
-    ldq, ldk, ldv = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    dev = _here(q, "q")
+    ldq, ldk, ldv = _heads(q, "q", dev), _heads(k, "k", dev), _heads(v, "v", dev)
     n, H, Dh = q.shape
-    Hkv = k.shape[1]
-    if n != plan.n_rows or k.shape[0] != plan.n_keys or v.shape != k.shape or k.shape[2] != Dh:
-        raise ValueError("q must have plan.n_rows rows, k and v plan.n_keys, of one head_dim")
-    if H == 0 or Hkv == 0 or H % Hkv:
-        raise ValueError("q's heads must be a multiple of k's")
-    R = 0
+    nk, Hkv, Dk = k.shape
+    if n != plan.n_rows or nk != plan.n_keys or v.shape != k.shape or Dk != Dh or plan.device != dev:
+        raise ValueError("q must have plan.n_rows rows, k and v plan.n_keys, of one head_dim, on "
+                         "the plan's device")
+    R = rel = 0
     if rel_bias is not None:
         if rel_bias.dim() != 2 or rel_bias.shape[1] % 2 == 0:
             raise ValueError("rel_bias must be [H, 2R + 1]")
         R = rel_bias.shape[1] // 2
-        _vec(rel_bias, "rel_bias", (H, 2 * R + 1))
-    _vec(slopes, "slopes", (H,))
+        rel = _vec(rel_bias, "rel_bias", (H, 2 * R + 1), dev)
+    slope = _vec(slopes, "slopes", (H,), dev)
     L = _lib.lib()
-    O = torch.empty(n, H * Dh, dtype=torch.bfloat16, device=q.device)
-    need = L.sj_attn_masked_workspace(C.byref(plan.info), H, Hkv, Dh)
-    if need < 0:
-        check(_lib.SJ_ERR_INVALID)
+    need = plan.workspace.get((H, Hkv, Dh))
+    if need is None:
+        need = L.sj_attn_masked_workspace(plan.info_ref, H, Hkv, Dh)
+        if need < 0:
+            check(_lib.SJ_ERR_INVALID)
+        plan.workspace[H, Hkv, Dh] = need
+    O = torch.empty((n, H * Dh), dtype=torch.bfloat16, device=q.device)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    args = _lib.AttnMaskedArgs(_at(q), _at(k), _at(v), _at(O), ldq, ldk, ldv, H * Dh, H, Hkv, Dh,
-                               Dh ** -0.5 if scale is None else scale, softcap, _at(rel_bias), R,
-                               _at(slopes))
-    check(L.sj_attn_masked(C.byref(args), C.byref(plan.info), _at(plan.data), _at(ws), need,
-                           _stream()))
+    args = _attn_masked_args(q.data_ptr(), k.data_ptr(), v.data_ptr(), O.data_ptr(), ldq, ldk, ldv,
+                             H * Dh, H, Hkv, Dh, Dh ** -0.5 if scale is None else scale, softcap,
+                             rel, R, slope)
+    rc = L.sj_attn_masked(args, plan.info_ref, plan.data.data_ptr(), _at(ws), need,
+                          _raw_stream(dev))
+    if rc:
+        check(rc)
     return O
 
 
@@ -266,8 +306,10 @@ class LoraPlan:
         check(L.sj_lora_plan(*a, None, 0, C.byref(self.info)))
         buf = np.empty(max(1, self.info.plan_len), np.int32)
         check(L.sj_lora_plan(*a, buf.ctypes.data, len(buf), C.byref(self.info)))
+        self.info_ref = C.byref(self.info)
         self.n_rows, self.rank, self.n_adapters = self.info.M, rank, n_adapters
         self.data = _plan_on_device(buf, device)
+        self.device = self.data.get_device()
 
 
 def gemm_lora(X, W, A, B, plan, *, scale=None, bias=None, act=0):
@@ -275,27 +317,25 @@ def gemm_lora(X, W, A, B, plan, *, scale=None, bias=None, act=0):
     in ``plan`` (rows without one: no such term).  X [M, K], W [N, K], A
     [n_adapters, rank, K], B [n_adapters, N, rank] bf16; scale [n_adapters] and
     bias [N] fp32; act as in :func:`gemm`."""
-    ldx = _rows(X, "X", torch.bfloat16)
-    for t, name in ((W, "W"), (A, "A"), (B, "B")):
-        _need(t, torch.bfloat16, name)
+    dev = _here(X, "X")
+    ldx = _rows(X, "X", torch.bfloat16, dev)
     M, K = X.shape
-    N = W.shape[0]
-    if M != plan.n_rows or tuple(W.shape) != (N, K):
-        raise ValueError("X must have plan.n_rows rows, and W the columns of X")
-    if tuple(A.shape) != (plan.n_adapters, plan.rank, K):
-        raise ValueError("A must be [n_adapters, rank, K]")
-    if tuple(B.shape) != (plan.n_adapters, N, plan.rank):
-        raise ValueError("B must be [n_adapters, N, rank]")
-    _vec(scale, "scale", (plan.n_adapters,))
-    _vec(bias, "bias", (N,))
+    N = W.shape[0] if W.dim() else 0
+    if M != plan.n_rows or plan.device != dev:
+        raise ValueError("X must have plan.n_rows rows, on the plan's device")
+    w = _vec(W, "W", (N, K), dev, torch.bfloat16)
+    a = _vec(A, "A", (plan.n_adapters, plan.rank, K), dev, torch.bfloat16)
+    b = _vec(B, "B", (plan.n_adapters, N, plan.rank), dev, torch.bfloat16)
+    s = _vec(scale, "scale", (plan.n_adapters,), dev)
+    bias_ = _vec(bias, "bias", (N,), dev)
     L = _lib.lib()
-    C_ = torch.empty(M, N, dtype=torch.bfloat16, device=X.device)
-    need = L.sj_gemm_lora_workspace(C.byref(plan.info), N, K)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=X.device)
-    args = _lib.GemmLoraArgs(_at(X), _at(W), _at(A), _at(B), _at(scale), _at(bias), _at(C_), ldx, N,
-                             N, K, act)
-    check(L.sj_gemm_lora(C.byref(args), C.byref(plan.info), _at(plan.data), _at(ws), need,
-                         _stream()))
+    need = L.sj_gemm_lora_workspace(plan.info_ref, N, K)
+    C_ = torch.empty((M, N), dtype=torch.bfloat16, device=X.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=X.device) if need else None
+    args = _gemm_lora_args(X.data_ptr(), w, a, b, s, bias_, C_.data_ptr(), ldx, N, N, K, act)
+    rc = L.sj_gemm_lora(args, plan.info_ref, plan.data.data_ptr(), _at(ws), need, _raw_stream(dev))
+    if rc:
+        check(rc)
     return C_
 
 
@@ -312,35 +352,41 @@ def norm_block(X, R, pre_w=None, pre_b=None, *, post_w=None, post_b=None, kind="
     gate: fp32 [D]; or, with cu (device int32 cumulative lengths), fp32
     [len(cu) - 1, D], a row for each segment; or [M, D] fp32 or bf16, through a
     sigmoid.  X' has X's type and is X itself with inplace; Y has out_dtype."""
-    if X.dtype not in _TYPES or R.dtype not in _TYPES or out_dtype not in _TYPES:
+    xt, rt, yt = _TYPES.get(X.dtype), _TYPES.get(R.dtype), _TYPES.get(out_dtype)
+    if xt is None or rt is None or yt is None:
         raise ValueError("X, R and Y must be float32 or bfloat16")
     if kind not in _KINDS:
         raise ValueError("kind must be 'ln' or 'rms'")
-    ldx, ldr = _rows(X, "X", X.dtype), _rows(R, "R", R.dtype)
-    M, D = X.shape
+    dev = _here(X, "X")
+    ldx, ldr = _rows(X, "X", X.dtype, dev), _rows(R, "R", R.dtype, dev)
     if R.shape != X.shape:
         raise ValueError("R must have X's shape")
-    for t, name in ((post_w, "post_w"), (post_b, "post_b"), (pre_w, "pre_w"), (pre_b, "pre_b")):
-        _vec(t, name, (D,))
-    mode = gtype = ldg = n_segs = 0
+    M, D = X.shape
+    d = (D,)
+    w1, b1 = _vec(post_w, "post_w", d, dev), _vec(post_b, "post_b", d, dev)
+    w2, b2 = _vec(pre_w, "pre_w", d, dev), _vec(pre_b, "pre_b", d, dev)
+    mode = gtype = ldg = n_segs = g = at = 0
     if gate is not None:
         if cu is not None:
             mode, n_segs = 2, cu.numel() - 1
-            _need(cu, torch.int32, "cu")
-            _vec(gate, "gate", (n_segs, D))
+            at = _vec(cu, "cu", (n_segs + 1,), dev, torch.int32)
+            g = _vec(gate, "gate", (n_segs, D), dev)
         elif gate.dim() == 1:
             mode = 1
-            _vec(gate, "gate", (D,))
+            g = _vec(gate, "gate", d, dev)
         else:
-            mode = 3
-            if gate.dtype not in _TYPES or gate.shape != X.shape:
+            mode, gtype = 3, _TYPES.get(gate.dtype)
+            if gtype is None or gate.shape != X.shape:
                 raise ValueError("gate must be [D], [segments, D] with cu, or [M, D]")
-            gtype, ldg = _TYPES[gate.dtype], _rows(gate, "gate", gate.dtype)
-    Xo = X if inplace else torch.empty(M, D, dtype=X.dtype, device=X.device)
-    Y = None if pre_w is None else torch.empty(M, D, dtype=out_dtype, device=X.device)
-    args = _lib.NormBlockArgs(_at(X), _at(Xo), _at(R), _at(Y), _TYPES[X.dtype], _TYPES[R.dtype],
-                              _TYPES[out_dtype], ldx, ldx if inplace else D, ldr, D, _at(post_w),
-                              _at(post_b), _at(pre_w), _at(pre_b), _KINDS[kind], eps, _at(gate),
-                              mode, gtype, ldg, _at(cu), n_segs, alpha, beta, M, D)
-    check(_lib.lib().sj_norm_block(C.byref(args), _stream()))
+            ldg, g = _rows(gate, "gate", gate.dtype, dev), gate.data_ptr()
+    # contiguous, and cheaper than torch.empty with a device
+    Xo = X if inplace else torch.empty_like(X, memory_format=torch.contiguous_format)
+    Y = None if pre_w is None else torch.empty_like(X, dtype=out_dtype,
+                                                    memory_format=torch.contiguous_format)
+    args = _norm_block_args(X.data_ptr(), Xo.data_ptr(), R.data_ptr(), _at(Y), xt, rt, yt, ldx,
+                            ldx if inplace else D, ldr, D, w1, b1, w2, b2, _KINDS[kind], eps, g,
+                            mode, gtype, ldg, at, n_segs, alpha, beta, M, D)
+    rc = _lib.lib().sj_norm_block(args, _raw_stream(dev))
+    if rc:
+        check(rc)
     return Xo, Y
