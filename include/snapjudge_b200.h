@@ -187,7 +187,12 @@ typedef struct sj_attn_plan_args {
   int n_q;
   int causal;
   int window;                /* >= 0; 0: none */
+  int form;                  /* SJ_ATTN_*: which form of the kernel the plan is for */
 } sj_attn_plan_args;
+
+#define SJ_ATTN_AUTO 0  /* by an estimate of what both would walk */
+#define SJ_ATTN_TILES 1 /* tiles of 128 query rows */
+#define SJ_ATTN_FEW 2   /* up to 16 query rows of a segment at a time */
 
 typedef struct sj_attn_plan_info {
   int64_t plan_len;  /* int32 words */
@@ -195,7 +200,12 @@ typedef struct sj_attn_plan_info {
   int32_t n_keys;    /* key rows */
   int32_t n_items;   /* tiles of up to 128 query rows */
   int32_t n_tiles;   /* 64-key tiles over all items */
-  int64_t off_items, off_tiles; /* word offsets into the plan */
+  int32_t longest;   /* key tiles of the longest item */
+  int32_t form;      /* SJ_ATTN_* */
+  /* few query rows: parts of groups of up to 16 rows, groups of more than one
+   * part, key tiles over all groups, rows of workspace that split groups take */
+  int32_t n_parts, n_splits, n_few_tiles, max_group_rows, ws_rows;
+  int64_t off_items, off_tiles, off_parts, off_splits, off_few_tiles; /* words into the plan */
 } sj_attn_plan_info;
 
 int sj_attn_plan(const sj_attn_plan_args* args, int32_t* plan, int64_t plan_len,
@@ -212,7 +222,8 @@ int sj_attn_plan(const sj_attn_plan_args* args, int32_t* plan, int64_t plan_len,
  * row pitches ldq, ldk, ldv, ldo in elements (q, k and v may be slices of one
  * packed tensor); H % Hkv == 0, head h reads key head h / (H / Hkv);
  * 1 <= Dh <= 128.  rel_bias fp32 [H, 2 rel_max + 1], slopes fp32 [H].
- * plan: the device copy of sj_attn_plan's.  Scores, softmax statistics and
+ * plan: the device copy of sj_attn_plan's; of the forms that it holds the one
+ * that should be faster for this head shape runs.  Scores, softmax statistics and
  * sums are fp32. */
 typedef struct sj_attn_masked_args {
   const sj_bf16 *q, *k, *v;

@@ -66,13 +66,17 @@ _F = C.c_float
 
 class AttnPlanArgs(C.Structure):
     _fields_ = [("cu_seqlens", _P), ("B", _I), ("docs", _P), ("n_docs", _I), ("prefix", _P),
-                ("kv_lens", _P), ("q_rows", _P), ("n_q", _I), ("causal", _I), ("window", _I)]
+                ("kv_lens", _P), ("q_rows", _P), ("n_q", _I), ("causal", _I), ("window", _I),
+                ("form", _I)]
 
 
 class AttnPlanInfo(C.Structure):
     _fields_ = [("plan_len", _L), ("n_rows", C.c_int32), ("n_keys", C.c_int32),
-                ("n_items", C.c_int32), ("n_tiles", C.c_int32), ("off_items", _L),
-                ("off_tiles", _L)]
+                ("n_items", C.c_int32), ("n_tiles", C.c_int32), ("longest", C.c_int32),
+                ("form", C.c_int32), ("n_parts", C.c_int32), ("n_splits", C.c_int32),
+                ("n_few_tiles", C.c_int32), ("max_group_rows", C.c_int32), ("ws_rows", C.c_int32),
+                ("off_items", _L), ("off_tiles", _L), ("off_parts", _L), ("off_splits", _L),
+                ("off_few_tiles", _L)]
 
 
 class AttnMaskedArgs(C.Structure):

@@ -1,0 +1,367 @@
+// attn_few.cu — masked attention for few query rows over many keys (head_dim 64
+// and 128): rows that ask for themselves (q_rows), and batches too small to fill
+// the GPU with tiles of 128 rows.
+//
+// K and V are read once for up to 16 query rows, so the bound is memory (16 KB
+// for each tile of 64 keys and key head at head_dim 64), and what has to be
+// arranged is loads in flight.  One warp does a part: up to 16 rows (times the
+// query heads that share a key head, 16 at a time) of one segment, for one key
+// head, over a run of the group's key tiles.  Nothing is staged in shared memory:
+//   S = Q K^T by mma.sync m16n8k16.  The sum over head dimensions may run in any
+//   order, so a thread's 16 bytes of a K row are taken as its operand words for
+//   two steps, and Q is permuted alike;
+//   O = P V: a thread loads 16 bytes (8 dimensions) of four key rows and pairs
+//   the keys with byte permutes; column n of output tile t is dimension 8 n + t
+//   (16 n + t at 128), so a thread ends up with whole runs of a row's dimensions.
+// (tcgen05 would multiply 128 rows for at most 16; the tensor pipe is idle either
+// way.)  Maximum and sum run online in fp32, P is rounded to bf16 as in the tile
+// kernel.  A group whose tiles are many is split into parts, whose maxima, sums
+// and outputs go to the workspace in fp32 and are joined, in order, by a second
+// kernel.  Rows whose output is not finite are computed again over their visible
+// keys alone.
+#include <algorithm>
+
+#include "attn_masked.cuh"
+#include "kernels.h"
+
+namespace sjb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh through one exponential: 1 - 2 / (1 + e^(2y)); absolute error about 2^-22
+__device__ __forceinline__ float tanh_exp(float y) {
+  return 1.f - __fdividef(2.f, 1.f + ex2f(y * (2.f * kLog2e)));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 load16(const bf16* p) {
+  return __ldg(reinterpret_cast<const uint4*>(p));
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+template <int DH>
+__global__ void __launch_bounds__(32 * kWarps) attn_few_kernel(const __grid_constant__ AttnMasked p, int mtiles,
+                                                               float* __restrict__ ws) {
+  constexpr int KC = DH == 64 ? 32 : 16;  // keys at a time
+  constexpr int NT = KC / 8;              // S tiles of 8 keys
+  constexpr int KL = DH / 32;             // 16-byte loads of a thread for a K row
+  constexpr int VL = DH / 64;             // ... for a V row
+  constexpr int OT = DH / 8;              // O tiles of 8 columns
+  const int lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
+  const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int hk = (int)(unit % p.Hkv);
+  const int64_t rest = unit / p.Hkv;
+  const int mt = (int)(rest % mtiles);
+  const int64_t part = rest / mtiles;
+  if (part >= p.n_parts) return;
+  const int4 pa = p.parts[2 * part], pb = p.parts[2 * part + 1];
+  const int row0 = pa.x, nrows = pa.y, tile0 = pa.z, ntiles = pa.w, ws_row = pb.x;
+  const int G = p.H / p.Hkv, M = nrows * G;
+  if (mt * 16 >= M) return;
+
+  // the thread's two rows (of 16): query row, head, position and intervals.  Rows
+  // past the end take the first one's and are not stored.
+  int mrow[2], mhead[2];
+  bool live[2];
+  int4 ra[2];
+  int b1[2];
+  uint32_t q[KL][2][4];  // 16 bytes of either row for each load
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int m = mt * 16 + gid + 8 * e;
+    live[e] = m < M;
+    const int mm = live[e] ? m : mt * 16;
+    mrow[e] = row0 + mm / G;
+    mhead[e] = hk * G + mm % G;
+    ra[e] = p.rows[2 * (int64_t)mrow[e]];
+    b1[e] = p.rows[2 * (int64_t)mrow[e] + 1].x;
+    const bf16* qp = p.q + (int64_t)mrow[e] * p.ldq + (int64_t)mhead[e] * DH + 8 * c;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const uint4 v = load16(qp + 32 * i);
+      q[i][e][0] = v.x, q[i][e][1] = v.y, q[i][e][2] = v.z, q[i][e][3] = v.w;
+    }
+  }
+  const bf16* kbase = p.k + (int64_t)hk * DH + 8 * c;
+  const bf16* vbase = p.v + (int64_t)hk * DH + (DH / 8) * gid;
+  const float scale2 = p.scale * kLog2e;
+  const float sy = p.cap > 0.f ? p.scale / p.cap : 0.f, cap2 = p.cap * kLog2e;
+  const int64_t rel_ld = 2 * (int64_t)p.rel_max + 1;
+
+  float m_ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[OT][4];
+#pragma unroll
+  for (int t = 0; t < OT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+
+  for (int tl = 0; tl < ntiles; ++tl) {
+    const int entry = p.few_tiles[tile0 + tl];
+    const int k0 = entry < 0 ? ~entry : entry;
+#pragma unroll 1
+    for (int kc = 0; kc < 64; kc += KC) {
+      const int kb = k0 + kc;
+      const bool mine = (kb < ra[0].z && kb + KC > ra[0].y) || (kb < b1[0] && kb + KC > ra[0].w) ||
+                        (kb < ra[1].z && kb + KC > ra[1].y) || (kb < b1[1] && kb + KC > ra[1].w);
+      if (!__any_sync(0xffffffffu, mine)) continue;  // no row sees these keys
+      // all loads of the step first: keys past the end (never visible) read the last row
+      uint4 kv[NT][KL], vv[NT / 2][4][VL];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int key = min(kb + 8 * t + gid, p.n_keys - 1);
+#pragma unroll
+        for (int i = 0; i < KL; ++i) kv[t][i] = load16(kbase + (int64_t)key * p.ldk + 32 * i);
+      }
+#pragma unroll
+      for (int s = 0; s < NT / 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = min(kb + 16 * s + 2 * c + (e & 1) + 8 * (e >> 1), p.n_keys - 1);
+#pragma unroll
+          for (int i = 0; i < VL; ++i) vv[s][e][i] = load16(vbase + (int64_t)key * p.ldv + 8 * i);
+        }
+      float x[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const uint32_t a0[4] = {q[i][0][0], q[i][1][0], q[i][0][1], q[i][1][1]};
+          const uint32_t a1[4] = {q[i][0][2], q[i][1][2], q[i][0][3], q[i][1][3]};
+          mma16816(x[t], a0, kv[t][i].x, kv[t][i].y);
+          mma16816(x[t], a1, kv[t][i].z, kv[t][i].w);
+        }
+      }
+      // x[t][2 e + f]: row e, key kb + 8 t + 2 c + f
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            const int j = kb + 8 * t + 2 * c + f;
+            float v = x[t][2 * e + f];
+            v = p.cap > 0.f ? cap2 * tanh_exp(v * sy) : v * scale2;
+            const int d = j - ra[e].x;
+            if (p.rel_bias) {
+              const float b =
+                  p.rel_bias[mhead[e] * rel_ld + min(max(d, -p.rel_max), p.rel_max) + p.rel_max];
+              v += fabsf(b) <= 3.402823466e38f
+                       ? fminf(fmaxf(b * kLog2e, -3.402823466e38f), 3.402823466e38f)
+                       : b;
+            }
+            if (p.slopes) v = fmaf(-p.slopes[mhead[e]] * kLog2e, fabsf((float)d), v);
+            const bool vis = (j >= ra[e].y && j < ra[e].z) || (j >= ra[e].w && j < b1[e]);
+            v = vis ? v : -INFINITY;
+            x[t][2 * e + f] = v;
+            mx[e] = fmaxf(mx[e], v);
+          }
+      float f2[2], mu[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float m = fmaxf(m_ref[e], quad_max(mx[e]));
+        mu[e] = m == -INFINITY ? 0.f : m;
+        f2[e] = ex2f(m_ref[e] - mu[e]);
+        m_ref[e] = m;
+        l[e] *= f2[e];
+      }
+      uint32_t pr[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p0 = ex2f(x[t][2 * e] - mu[e]), p1 = ex2f(x[t][2 * e + 1] - mu[e]);
+          l[e] += p0 + p1;  // this thread's keys; the quad is added up at the end
+          pr[t][e] = pack_bf16(p0, p1);
+        }
+#pragma unroll
+      for (int t = 0; t < OT; ++t) {
+        o[t][0] *= f2[0];
+        o[t][1] *= f2[0];
+        o[t][2] *= f2[1];
+        o[t][3] *= f2[1];
+      }
+#pragma unroll
+      for (int s = 0; s < NT / 2; ++s) {
+        const uint32_t a[4] = {pr[2 * s][0], pr[2 * s][1], pr[2 * s + 1][0], pr[2 * s + 1][1]};
+#pragma unroll
+        for (int t = 0; t < OT; ++t) {
+          const int i = t >> 3, w = (t & 7) >> 1;
+          const uint32_t sel = t & 1 ? 0x7632 : 0x5410;
+          mma16816(o[t], a, __byte_perm(word(vv[s][0][i], w), word(vv[s][1][i], w), sel),
+                   __byte_perm(word(vv[s][2][i], w), word(vv[s][3][i], w), sel));
+        }
+      }
+    }
+  }
+
+  // row e of the thread: dimensions 2 c (DH / 8) + [0, DH / 4), the first half of
+  // them in o[.][2 e], the second in o[.][2 e + 1]
+#pragma unroll
+  for (int e = 0; e < 2; ++e) l[e] = quad_sum(l[e]);
+  if (ws_row >= 0) {  // a part: maximum, sum and output for the join
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (!live[e]) continue;
+      float* w = ws + ((int64_t)(ws_row + mrow[e] - row0) * p.H + mhead[e]) * (DH + 4);
+      if (c == 0) {
+        w[DH] = m_ref[e];
+        w[DH + 1] = l[e];
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int t = 0; t < OT; t += 4)
+          *reinterpret_cast<float4*>(w + (2 * c + hh) * (DH / 8) + t) =
+              make_float4(o[t][2 * e + hh], o[t + 1][2 * e + hh], o[t + 2][2 * e + hh],
+                          o[t + 3][2 * e + hh]);
+    }
+    return;
+  }
+  bool odd[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    // no visible key, or only scores of -inf: 0 (a NaN in l stays one)
+    const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
+    float chk = 0.f;
+    bf16* out = p.O + (int64_t)mrow[e] * p.ldo + (int64_t)mhead[e] * DH + 2 * c * (DH / 8);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int t = 0; t < OT; t += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = o[t + i][2 * e + hh] * inv;
+          chk = fmaf(v[i], 0.f, chk);
+        }
+        if (live[e])
+          *reinterpret_cast<uint4*>(out + hh * (DH / 8) + t) =
+              make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                         pack_bf16(v[6], v[7]));
+      }
+    odd[e] = chk != 0.f && live[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    unsigned again = __ballot_sync(0xffffffffu, odd[e]);
+    while (again) {
+      const int src = (__ffs(again) - 1) & ~3;  // a quad holds one row
+      again &= ~(15u << src);
+      const int row = __shfl_sync(0xffffffffu, mrow[e], src);
+      const int h = __shfl_sync(0xffffffffu, mhead[e], src);
+      float r[4];
+      attn_masked_row(p, row, h, lane, r);
+      bf16* out = p.O + (int64_t)row * p.ldo + (int64_t)h * DH;
+#pragma unroll
+      for (int d = 0; d < DH / 32; ++d) out[lane + 32 * d] = __float2bfloat16(r[d]);
+    }
+  }
+}
+
+// One warp joins the parts of a (row, head), in order.
+template <int DH>
+__global__ void __launch_bounds__(32 * kWarps) attn_few_join(const __grid_constant__ AttnMasked p,
+                                                             const float* __restrict__ ws) {
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int h = (int)(unit % p.H);
+  const int64_t rest = unit / p.H;
+  const int r = (int)(rest % 16);
+  const int64_t grp = rest / 16;
+  if (grp >= p.n_splits) return;
+  const int4 g = p.splits[grp];  // first row, rows, parts, first workspace row
+  if (r >= g.y) return;
+  constexpr int E = DH / 32;
+  // lane k takes part k's maximum and sum (32 parts at a time), then every lane
+  // adds its dimensions over the parts: no load waits for another part's
+  const float* base = ws + ((int64_t)(g.w + r) * p.H + h) * (DH + 4);
+  const int64_t step = (int64_t)g.y * p.H * (DH + 4);
+  float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = 0.f;
+  for (int k = lane; k < g.z; k += 32) m = fmaxf(m, base[k * step + DH]);
+  m = warp_max(m);
+  const float mu = m == -INFINITY ? 0.f : m;
+  for (int k0 = 0; k0 < g.z; k0 += 32) {
+    const int k = k0 + lane;
+    const float f = k < g.z ? ex2f(base[k * step + DH] - mu) : 0.f;
+    l += k < g.z ? base[k * step + DH + 1] * f : 0.f;
+    const int n = min(32, g.z - k0);
+#pragma unroll 4
+    for (int e = 0; e < n; ++e) {
+      const float fe = __shfl_sync(0xffffffffu, f, e);
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] += fe * base[(k0 + e) * step + lane + 32 * i];
+    }
+  }
+  l = warp_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  bf16* out = p.O + (int64_t)(g.x + r) * p.ldo + (int64_t)h * DH;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    o[i] *= inv;
+    odd = odd || !(fabsf(o[i]) <= 3.402823466e38f);
+  }
+  if (__any_sync(0xffffffffu, odd)) {
+    float v[4];
+    attn_masked_row(p, g.x + r, h, lane, v);
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) out[lane + 32 * i] = __float2bfloat16(o[i]);
+}
+
+template <int DH>
+cudaError_t launch(const AttnMasked& p, float* ws, cudaStream_t st) {
+  const int mtiles = (std::min(16, p.max_group_rows) * (p.H / p.Hkv) + 15) / 16;
+  const int64_t units = (int64_t)p.n_parts * mtiles * p.Hkv;
+  const int64_t blocks = (units + kWarps - 1) / kWarps;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  attn_few_kernel<DH><<<(unsigned)blocks, 32 * kWarps, 0, st>>>(p, mtiles, ws);
+  if (cudaError_t rc = cudaGetLastError()) return rc;
+  if (p.n_splits == 0) return cudaSuccess;
+  const int64_t jb = ((int64_t)p.n_splits * 16 * p.H + kWarps - 1) / kWarps;
+  if (jb > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  attn_few_join<DH><<<(unsigned)jb, 32 * kWarps, 0, st>>>(p, ws);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t attn_few(const AttnMasked& p, void* ws, cudaStream_t st) {
+  float* w = static_cast<float*>(ws);
+  return p.Dh == 64 ? launch<64>(p, w, st) : launch<128>(p, w, st);
+}
+
+}  // namespace sjb

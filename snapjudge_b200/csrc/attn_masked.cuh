@@ -21,6 +21,11 @@ struct AttnMasked {
   const int4* rows;           // plan: 2 x int4 for each query row
   const int4* items;          // plan: one for each query tile
   const int32_t* tiles;       // plan: key tiles
+  // plan, few query rows (n_parts > 0): 2 x int4 for each part, one for each split
+  // group, and the parts' key tiles
+  int n_parts, n_splits, max_group_rows;
+  const int4 *parts, *splits;
+  const int32_t* few_tiles;
 };
 
 inline AttnMasked attn_masked_params(const sj_attn_masked_args& a, const sj_attn_plan_info& info,
@@ -49,6 +54,12 @@ inline AttnMasked attn_masked_params(const sj_attn_masked_args& a, const sj_attn
   p.rows = reinterpret_cast<const int4*>(plan);
   p.items = reinterpret_cast<const int4*>(plan + info.off_items);
   p.tiles = plan + info.off_tiles;
+  p.n_parts = info.n_parts;
+  p.n_splits = info.n_splits;
+  p.max_group_rows = info.max_group_rows;
+  p.parts = reinterpret_cast<const int4*>(plan + info.off_parts);
+  p.splits = reinterpret_cast<const int4*>(plan + info.off_splits);
+  p.few_tiles = plan + info.off_few_tiles;
   return p;
 }
 
@@ -114,7 +125,9 @@ cudaError_t attn_masked_simt(const AttnMasked& p, cudaStream_t st);
 // tcgen05 kernel (attn_masked_tc.cu)
 bool attn_masked_tc_supported(const AttnMasked& p);
 cudaError_t attn_masked_tc(const AttnMasked& p, cudaStream_t st);
-// As attn_tc_take_status, for this kernel.
+// For few query rows (attn_few.cu); same requirements, plan with parts.
+cudaError_t attn_few(const AttnMasked& p, void* workspace, cudaStream_t st);
+// As attn_tc_take_status, for attn_masked_tc.
 cudaError_t attn_masked_take_status(int* code);
 
 }  // namespace sjb

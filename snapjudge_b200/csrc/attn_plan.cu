@@ -12,7 +12,16 @@
 //   tiles  for each item its key tiles: the first key row k0 of 64, greedily
 //          from the first key that a row of the item sees and no earlier tile
 //          covers; ~k0 when every row of the item sees all 64 keys (no mask).
+// For few query rows also
+//   parts   8 words each: first row, rows, first key tile, key tiles of a run of a
+//           group's tiles, the workspace row of its first row (-1: the group has
+//           one part), 3 words of padding; a group is up to 16 query rows of one
+//           segment;
+//   splits  4 words for each group of several parts: first row, rows, parts, first
+//           workspace row;
+//   few     the groups' key tiles, as above.
 #include <algorithm>
+#include <array>
 #include <new>
 #include <vector>
 
@@ -29,12 +38,41 @@ int bad(const char* m) {
 struct Iv {
   int a, b;
 };
+// Above this many query rows the tile kernel fills the GPU.
+constexpr int kFewMostRows = 4096;
+
+// The rows' keys as tiles: `next` tiles greedily over the union of the intervals.
+struct Row {
+  int pos, a0, a1, b0, b1, seg;
+};
+void cover(const Row* rows, int r0, int r1, std::vector<Iv>& iv, std::vector<int32_t>& tiles) {
+  iv.clear();
+  Iv ca{0, 0x7fffffff}, cb{0, 0x7fffffff};  // keys that every row sees, by its intervals
+  for (int r = r0; r < r1; ++r) {
+    const Row& w = rows[r];
+    if (w.a1 > w.a0) iv.push_back({w.a0, w.a1});
+    if (w.b1 > w.b0) iv.push_back({w.b0, w.b1});
+    ca.a = std::max(ca.a, w.a0), ca.b = std::min(ca.b, w.a1);
+    cb.a = std::max(cb.a, w.b0), cb.b = std::min(cb.b, w.b1);
+  }
+  std::sort(iv.begin(), iv.end(), [](const Iv& x, const Iv& y) { return x.a < y.a; });
+  long long next = 0;  // first key that no tile covers yet
+  for (const Iv& v : iv) {
+    for (long long k = std::max<long long>(v.a, next); k < v.b; k = next) {
+      next = k + 64;
+      const int k0 = (int)k;
+      const bool full = (k0 >= ca.a && next <= ca.b) || (k0 >= cb.a && next <= cb.b);
+      tiles.push_back(full ? ~k0 : k0);
+    }
+  }
+}
 
 int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
               sj_attn_plan_info* info) {
   const int32_t* cu = p.cu_seqlens;
   if (p.B < 0) return bad("negative batch");
   if (p.window < 0) return bad("negative window");
+  if (p.form < SJ_ATTN_AUTO || p.form > SJ_ATTN_FEW) return bad("bad form");
   if (!cu) return bad("cu_seqlens is null");
   if (cu[0] != 0) return bad("cu_seqlens[0] must be 0");
   for (int b = 0; b < p.B; ++b) {
@@ -64,9 +102,6 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
   const int nr = p.q_rows ? p.n_q : T;
 
   // the rows' intervals
-  struct Row {
-    int pos, a0, a1, b0, b1;
-  };
   std::vector<Row> rows((size_t)nr);
   for (int r = 0, b = 0, d = 0; r < nr; ++r) {
     const int i = p.q_rows ? p.q_rows[r] : r;
@@ -91,6 +126,7 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
     hi = std::max(hi, lo);
     Row& w = rows[r];
     w.pos = i;
+    w.seg = b;
     if (a1 == a0) {  // no prefix
       w.a0 = lo, w.a1 = hi, w.b0 = w.b1 = hi;
     } else if (lo == a1) {  // one interval
@@ -109,27 +145,8 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
   std::vector<Iv> iv;
   for (int r0 = 0; r0 < nr; r0 += 128) {
     const int r1 = std::min(nr, r0 + 128);
-    iv.clear();
-    Iv ca{0, 0x7fffffff}, cb{0, 0x7fffffff};  // keys that every row sees, by its intervals
-    for (int r = r0; r < r1; ++r) {
-      const Row& w = rows[r];
-      if (w.a1 > w.a0) iv.push_back({w.a0, w.a1});
-      if (w.b1 > w.b0) iv.push_back({w.b0, w.b1});
-      ca.a = std::max(ca.a, w.a0), ca.b = std::min(ca.b, w.a1);
-      cb.a = std::max(cb.a, w.b0), cb.b = std::min(cb.b, w.b1);
-    }
-    std::sort(iv.begin(), iv.end(), [](const Iv& x, const Iv& y) { return x.a < y.a; });
     Item it{r0, r1 - r0, (int)tiles.size(), 0};
-    long long next = 0;  // first key that no tile covers yet
-    for (const Iv& v : iv) {
-      for (long long k = std::max<long long>(v.a, next); k < v.b; k = next) {
-        next = k + 64;
-        const int k0 = (int)k;
-        const bool full =
-            (k0 >= ca.a && next <= ca.b) || (k0 >= cb.a && next <= cb.b);
-        tiles.push_back(full ? ~k0 : k0);
-      }
-    }
+    cover(rows.data(), r0, r1, iv, tiles);
     if (tiles.size() > 0x7fffffff) return bad("the batch needs too many key tiles");
     it.tiles = (int)tiles.size() - it.tile0;
     items.push_back(it);
@@ -137,13 +154,56 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
   std::stable_sort(items.begin(), items.end(),
                    [](const Item& x, const Item& y) { return x.tiles > y.tiles; });
 
+  // few query rows: groups of up to 16 rows of one segment, split into parts
+  struct Part {
+    int row0, rows, tile0, tiles, ws;
+  };
+  std::vector<Part> parts;
+  std::vector<std::array<int, 4>> splits;
+  std::vector<int32_t> few;
+  int max_rows = 0;
+  long long ws_rows = 0;
+  if (nr > 0 && (p.form == SJ_ATTN_FEW || (p.form == SJ_ATTN_AUTO && nr <= kFewMostRows))) {
+    std::vector<Item> groups;
+    for (int r0 = 0, r1; r0 < nr; r0 = r1) {
+      for (r1 = r0 + 1; r1 < nr && r1 < r0 + 16 && rows[r1].seg == rows[r0].seg;) ++r1;
+      Item g{r0, r1 - r0, (int)few.size(), 0};
+      cover(rows.data(), r0, r1, iv, few);
+      g.tiles = (int)few.size() - g.tile0;
+      groups.push_back(g);
+    }
+    // parts short enough to spread over the SMs, long enough not to be joined often
+    const int most = (int)std::min<long long>(8, 1 + (long long)few.size() * 8 / (148 * 8));
+    for (const Item& g : groups) {
+      const int n = std::max(1, (g.tiles + most - 1) / most), per = (g.tiles + n - 1) / n;
+      max_rows = std::max(max_rows, g.rows);
+      if (n > 1) splits.push_back({g.row0, g.rows, n, (int)ws_rows});
+      for (int k = 0; k < n; ++k) {
+        const int t0 = std::min(g.tiles, k * per), t1 = std::min(g.tiles, t0 + per);
+        parts.push_back({g.row0, g.rows, g.tile0 + t0, t1 - t0, n > 1 ? (int)ws_rows : -1});
+        if (n > 1) ws_rows += g.rows;
+      }
+    }
+  }
+
   info->n_rows = nr;
   info->n_keys = T;
   info->n_items = (int)items.size();
   info->n_tiles = (int)tiles.size();
   info->off_items = 8ll * nr;
   info->off_tiles = info->off_items + 4ll * (long long)items.size();
-  info->plan_len = info->off_tiles + (long long)tiles.size();
+  info->n_parts = (int)parts.size();
+  info->n_splits = (int)splits.size();
+  info->n_few_tiles = (int)few.size();
+  info->longest = items.empty() ? 0 : items[0].tiles;
+  info->form = p.form;
+  info->max_group_rows = max_rows;
+  info->ws_rows = (int)ws_rows;
+  info->off_parts = info->off_tiles + ((long long)tiles.size() + 3) / 4 * 4;  // 16-byte words
+  info->off_splits = info->off_parts + 8ll * (long long)parts.size();
+  info->off_few_tiles = info->off_splits + 4ll * (long long)splits.size();
+  info->plan_len = parts.empty() ? info->off_tiles + (long long)tiles.size()
+                                 : info->off_few_tiles + (long long)few.size();
   if (!plan) return SJ_OK;
   if (plan_len < info->plan_len) return bad("the plan's memory is too small");
   for (int r = 0; r < nr; ++r) {
@@ -156,6 +216,16 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
     std::copy(v, v + 4, plan + info->off_items + 4 * (long long)k);
   }
   std::copy(tiles.begin(), tiles.end(), plan + info->off_tiles);
+  if (parts.empty()) return SJ_OK;
+  std::fill(plan + info->off_tiles + (long long)tiles.size(), plan + info->off_parts, 0);
+  for (size_t k = 0; k < parts.size(); ++k) {
+    const Part& q = parts[k];
+    const int32_t v[8] = {q.row0, q.rows, q.tile0, q.tiles, q.ws, 0, 0, 0};
+    std::copy(v, v + 8, plan + info->off_parts + 8 * (long long)k);
+  }
+  for (size_t k = 0; k < splits.size(); ++k)
+    std::copy(splits[k].begin(), splits[k].end(), plan + info->off_splits + 4 * (long long)k);
+  std::copy(few.begin(), few.end(), plan + info->off_few_tiles);
   return SJ_OK;
 }
 

@@ -197,6 +197,9 @@ _gemm_lora_args = _packer(_lib.GemmLoraArgs)
 _norm_block_args = _packer(_lib.NormBlockArgs)
 
 
+_FORMS = {"auto": 0, "tiles": 1, "few": 2}
+
+
 class AttnPlan:
     """Which keys each query row of a packed batch sees, for :func:`attn_masked`.
 
@@ -207,10 +210,14 @@ class AttnPlan:
     ``docs``: host row boundaries of the documents, a refinement of ``cu``
     (None: a segment is one document); ``prefix``, ``kv_lens``: host [B] or None;
     ``q_rows``: strictly increasing packed rows that ask (None: all).
+    ``form``: "tiles" of 128 query rows, "few" (up to 16 rows of a segment at a
+    time), or "auto", the one that should be faster.
     """
 
     def __init__(self, cu, *, docs=None, prefix=None, kv_lens=None, q_rows=None, causal=False,
-                 window=0, device=None):
+                 window=0, form="auto", device=None):
+        if form not in _FORMS:
+            raise ValueError("form must be 'auto', 'tiles' or 'few'")
         cu = _host_i32(cu, "cu")
         docs, prefix = _host_i32(docs, "docs"), _host_i32(prefix, "prefix")
         kv_lens, q_rows = _host_i32(kv_lens, "kv_lens"), _host_i32(q_rows, "q_rows")
@@ -225,7 +232,7 @@ class AttnPlan:
         p = lambda a: None if a is None else a.ctypes.data  # noqa: E731
         args = _lib.AttnPlanArgs(p(cu), B, p(docs), 0 if docs is None else len(docs) - 1, p(prefix),
                                  p(kv_lens), p(q_rows), 0 if q_rows is None else len(q_rows),
-                                 int(causal), int(window))
+                                 int(causal), int(window), _FORMS[form])
         self.info = _lib.AttnPlanInfo()
         L = _lib.lib()
         check(L.sj_attn_plan(C.byref(args), None, 0, C.byref(self.info)))

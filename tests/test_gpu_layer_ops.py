@@ -100,12 +100,15 @@ def close(got, want, tol):
                            f"{float(((got.double() - want).abs() / tol).max()):.3g} tolerances")
 
 
-def plan_of(m):
-    return ops.AttnPlan(m["cu"], **{k: v for k, v in m.items() if k != "cu"})
+def plan_of(m, form="auto"):
+    return ops.AttnPlan(m["cu"], form=form, **{k: v for k, v in m.items() if k != "cu"})
 
 
-def check_attn(m, H, Hkv, Dh, seed=1, qscale=1.0, **kw):
-    plan = plan_of(m)
+both_forms = pytest.mark.parametrize("form", ["tiles", "few"])
+
+
+def check_attn(m, H, Hkv, Dh, form, seed=1, qscale=1.0, **kw):
+    plan = plan_of(m, form)
     g = gen(seed)
     q = rnd((plan.n_rows, H, Dh), g, qscale)
     k, v = rnd((plan.n_keys, Hkv, Dh), g), rnd((plan.n_keys, Hkv, Dh), g)
@@ -143,8 +146,9 @@ MASKS = {
 
 @pytest.mark.parametrize("name", MASKS)
 @pytest.mark.parametrize("H,Hkv,Dh", [(3, 3, 64), (4, 2, 128), (2, 1, 16)])
-def test_attn_masks(name, H, Hkv, Dh):
-    check_attn(MASKS[name], H, Hkv, Dh)
+@both_forms
+def test_attn_masks(name, H, Hkv, Dh, form):
+    check_attn(MASKS[name], H, Hkv, Dh, form)
 
 
 MODS = [dict(softcap=30.0, qscale=6.0), dict(softcap=2.0, qscale=9.0), dict(rel=32), dict(rel=0),
@@ -155,30 +159,33 @@ MODS = [dict(softcap=30.0, qscale=6.0), dict(softcap=2.0, qscale=9.0), dict(rel=
 @pytest.mark.parametrize("mods", MODS, ids=str)
 @pytest.mark.parametrize("name", ["long", "state and questions", "everything", "few rows ask"])
 @pytest.mark.parametrize("H,Hkv,Dh", [(3, 3, 64), (4, 1, 128), (2, 2, 32)])
-def test_attn_scores(name, mods, H, Hkv, Dh):
-    check_attn(MASKS[name], H, Hkv, Dh, seed=2, **mods)
+@both_forms
+def test_attn_scores(name, mods, H, Hkv, Dh, form):
+    check_attn(MASKS[name], H, Hkv, Dh, form, seed=2, **mods)
 
 
 @pytest.mark.parametrize("Dh", [1, 7, 8, 40, 80, 96, 100])
 def test_attn_other_head_dims(Dh):
-    check_attn(MASKS["state and questions"], 2, 2, Dh, seed=3, rel=16)
+    check_attn(MASKS["state and questions"], 2, 2, Dh, "auto", seed=3, rel=16)
 
 
 @pytest.mark.parametrize("H,Hkv", [(16, 1), (12, 3), (5, 5)])
 @pytest.mark.parametrize("name", ["long", "few rows ask"])
-def test_attn_shared_heads(name, H, Hkv):
-    check_attn(MASKS[name], H, Hkv, 64, seed=4, slope=True)
+@both_forms
+def test_attn_shared_heads(name, H, Hkv, form):
+    check_attn(MASKS[name], H, Hkv, 64, form, seed=4, slope=True)
 
 
 @pytest.mark.parametrize("Dh", [64, 128, 16])
 @pytest.mark.parametrize("name", ["short and empty segments", "short keys", "state and questions",
                                   "everything", "few rows ask", "window"])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
-def test_attn_masked_places_never_reach_the_output(name, value, Dh):
+@both_forms
+def test_attn_masked_places_never_reach_the_output(name, value, Dh, form):
     """A key that some rows do not see: what it holds changes only the rows that
     see it."""
     m = MASKS[name]
-    plan = plan_of(m)
+    plan = plan_of(m, form)
     ok, _ = sees(m)
     g = gen(5)
     H = 2
@@ -196,11 +203,12 @@ def test_attn_masked_places_never_reach_the_output(name, value, Dh):
 
 
 @pytest.mark.parametrize("Dh", [64, 128, 16])
-def test_attn_rows_of_lowest_scores(Dh):
+@both_forms
+def test_attn_rows_of_lowest_scores(Dh, form):
     """A bias of the type's lowest value is a score like any other: a row whose
     every key has it weighs them alike; one whose every score is -inf gives 0."""
     m = dict(cu=cum([150, 90]))
-    plan = plan_of(m)
+    plan = plan_of(m, form)
     g = gen(6)
     q, k, v = (rnd((240, 1, Dh), g) for _ in range(3))
     low = torch.full((1, 1), torch.finfo(F32).min, device=DEV)
@@ -219,11 +227,12 @@ def test_attn_rows_of_lowest_scores(Dh):
 @pytest.mark.parametrize("Dh", [64, 128])
 @pytest.mark.parametrize("pad", [0, 8, 1])
 @pytest.mark.parametrize("name", ["state and questions", "few rows ask"])
-def test_attn_strides_and_alignment(name, pad, Dh):
+@both_forms
+def test_attn_strides_and_alignment(name, pad, Dh, form):
     """Slices of a packed tensor, row pitches that are no multiple of 16 bytes,
     and tensors that start anywhere give what contiguous ones give."""
     m = MASKS[name]
-    plan = plan_of(m)
+    plan = plan_of(m, form)
     H, Hkv, T = 4, 2, plan.n_keys
     g = gen(7)
     flat = rnd((T, (H + 2 * Hkv) * Dh + pad), g)
@@ -237,7 +246,8 @@ def test_attn_strides_and_alignment(name, pad, Dh):
     close(ops.attn_masked(q, k, v, plan), *ref_attn(q, k, v, m))
 
 
-def test_attn_offsets_past_32_bits():
+@both_forms
+def test_attn_offsets_past_32_bits(form):
     """Key rows a million elements apart: offsets above 2^31 elements."""
     T, Dh = 2300, 64
     g = gen(8)
@@ -245,16 +255,17 @@ def test_attn_offsets_past_32_bits():
     kv = big.as_strided((T, 2, Dh), (1 << 20, Dh, 1))
     kv.copy_(rnd((T, 2, Dh), g))
     for m in (dict(cu=[0, 2000, T], q_rows=[3, 2299]), dict(cu=[0, 2000, T])):
-        plan = plan_of(m)
+        plan = plan_of(m, form)
         q = rnd((plan.n_rows, 1, Dh), g)
         close(ops.attn_masked(q, kv[:, :1], kv[:, 1:], plan),
               *ref_attn(q, kv[:, :1], kv[:, 1:], m))
 
 
-def test_attn_many_short_segments_and_repeatable():
+@both_forms
+def test_attn_many_short_segments_and_repeatable(form):
     lens = np.random.default_rng(9).integers(0, 90, 900)
     m = dict(cu=cum(lens))
-    plan = plan_of(m)
+    plan = plan_of(m, form)
     g = gen(9)
     q, k, v = (rnd((plan.n_keys, 2, 64), g) for _ in range(3))
     got = ops.attn_masked(q, k, v, plan)
@@ -266,10 +277,11 @@ def test_attn_many_short_segments_and_repeatable():
         close(got[rows], *ref_attn(q[rows], k[rows], v[rows], sub))
 
 
-def test_attn_long_rows_keep_their_sum():
+@both_forms
+def test_attn_long_rows_keep_their_sum(form):
     """One row over 60,000 keys of equal score: the mean of the values."""
     T = 60000
-    plan = ops.AttnPlan([0, T], q_rows=[T - 1])
+    plan = ops.AttnPlan([0, T], q_rows=[T - 1], form=form)
     v = rnd((T, 1, 64), gen(10))
     got = ops.attn_masked(torch.zeros(1, 1, 64, dtype=BF, device=DEV), rnd((T, 1, 64), gen(11)), v,
                           plan)
@@ -277,9 +289,10 @@ def test_attn_long_rows_keep_their_sum():
     close(got, want, 2.0 ** -8 * want.abs() + 2.0 ** -8 * v.double().abs().mean(0) / 100)
 
 
-def test_attn_on_another_stream():
+@both_forms
+def test_attn_on_another_stream(form):
     m = MASKS["state and questions"]
-    plan = plan_of(m)
+    plan = plan_of(m, form)
     g = gen(12)
     q, k, v = (rnd((plan.n_keys, 3, 64), g) for _ in range(3))
     want = ops.attn_masked(q, k, v, plan)
@@ -305,6 +318,7 @@ def test_attn_python_refusals():
                 lambda: ops.attn_masked(q.cpu(), q, q, plan),
                 lambda: ops.AttnPlan([0, 10], prefix=[1, 2]),
                 lambda: ops.AttnPlan([0, 10.5]),
+                lambda: ops.AttnPlan([0, 10], form="both"),
                 lambda: ops.AttnPlan([0, 2 ** 31])):
         with pytest.raises((ValueError, RuntimeError)):
             bad()

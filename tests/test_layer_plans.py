@@ -18,11 +18,11 @@ def _i32(a):
     return None if a is None else np.ascontiguousarray(a, np.int32)
 
 
-def attn_plan(cu, docs=None, prefix=None, kv_lens=None, q_rows=None, causal=0, window=0):
+def attn_plan(cu, docs=None, prefix=None, kv_lens=None, q_rows=None, causal=0, window=0, form=0):
     cu, docs, prefix, kv_lens, q_rows = map(_i32, (cu, docs, prefix, kv_lens, q_rows))
     a = _lib.AttnPlanArgs(_p(cu), len(cu) - 1, _p(docs), 0 if docs is None else len(docs) - 1,
                           _p(prefix), _p(kv_lens), _p(q_rows), 0 if q_rows is None else len(q_rows),
-                          causal, window)
+                          causal, window, form)
     info = _lib.AttnPlanInfo()
     L = _lib.lib()
     rc = L.sj_attn_plan(C.byref(a), None, 0, C.byref(info))
@@ -92,7 +92,7 @@ def test_attn_plan_shows_the_defined_keys(case):
     assert (got == want).all()
     # items: every query row in one; their key tiles cover what the rows see, once
     items = plan[info.off_items:info.off_tiles].reshape(-1, 4)
-    tiles = plan[info.off_tiles:]
+    tiles = plan[info.off_tiles:info.off_tiles + info.n_tiles]
     seen = np.zeros(info.n_rows, int)
     assert (np.diff(items[:, 3]) <= 0).all()  # longest first
     for row0, n, t0, nt in items:
@@ -110,7 +110,48 @@ def test_attn_plan_shows_the_defined_keys(case):
     assert (seen == 1).all()
 
 
+@pytest.mark.parametrize("case", CASES + [dict(cu=[0, 5000], q_rows=[17, 4000])])
+def test_attn_plan_parts_of_few_rows(case):
+    """Every query row is in one group, whose parts' tiles cover what it sees,
+    once; groups of several parts have workspace rows of their own."""
+    want = visible(**case)
+    rc, info, plan = attn_plan(form=2, **case)
+    assert rc == 0
+    if info.n_rows == 0:
+        assert info.n_parts == 0
+        return
+    seg = np.repeat(np.arange(len(case["cu"]) - 1), np.diff(case["cu"]))
+    pos = plan[:8 * info.n_rows].reshape(-1, 8)[:, 0]
+    parts = plan[info.off_parts:info.off_splits].reshape(-1, 8)[:, :5]
+    splits = {s[0]: s for s in plan[info.off_splits:info.off_few_tiles].reshape(-1, 4).tolist()}
+    tiles = plan[info.off_few_tiles:]
+    assert len(tiles) == info.n_few_tiles
+    assert len(parts) == info.n_parts and len(splits) == info.n_splits
+    groups, ws = {}, np.zeros(info.ws_rows, int)
+    for row0, n, t0, nt, w in parts:
+        assert 1 <= n <= min(16, info.max_group_rows) and len(set(seg[pos[row0:row0 + n]])) == 1
+        groups.setdefault((row0, n), []).append((t0, nt, w))
+        if w >= 0:
+            ws[w:w + n] += 1
+    assert (ws == 1).all()
+    assert sorted(r for row0, n in groups for r in range(row0, row0 + n)) == list(range(info.n_rows))
+    for (row0, n), mine in groups.items():
+        assert (len(mine) > 1) == (row0 in splits)
+        if len(mine) > 1:
+            assert splits[row0] == [row0, n, len(mine), mine[0][2]]
+            assert [w for _, _, w in mine] == [mine[0][2] + k * n for k in range(len(mine))]
+        else:
+            assert mine[0][2] == -1
+        cover = np.zeros(want.shape[1] + 64, int)
+        for t0, nt, _ in mine:
+            for t in tiles[t0:t0 + nt]:
+                cover[(~t if t < 0 else t):][:64] += 1
+        assert cover.max(initial=0) <= 1
+        assert (cover[:want.shape[1]][want[row0:row0 + n].any(0)] == 1).all()
+
+
 @pytest.mark.parametrize("case,word", [
+    (dict(cu=[0, 5], form=3), b"form"),
     (dict(cu=[1, 5]), b"cu_seqlens[0]"),
     (dict(cu=[0, 5, 3]), b"non-decreasing"),
     (dict(cu=[0, 5], window=-1), b"window"),
