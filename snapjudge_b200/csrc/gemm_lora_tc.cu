@@ -62,9 +62,10 @@ __device__ __forceinline__ void fence_async_global() {
 }
 
 // ---- U = scale_a X A_a^T -------------------------------------------------------
-// One CTA: 128 rows, up to 16 slabs (N = 256).  Thread 0 loads, thread 32 issues
-// the MMAs, all four warps write U (thread = row).
-constexpr int kShrinkStages = 4;
+// One CTA: 128 rows, up to 8 slabs (N = 128); 96 KB of stages, so that two share
+// an SM.  Thread 0 loads, thread 32 issues the MMAs, all four warps write U
+// (thread = row).
+constexpr int kShrinkStages = 3, kShrinkSlabs = 8;
 
 __global__ void __launch_bounds__(128)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap mapX,
@@ -74,9 +75,10 @@ __global__ void __launch_bounds__(128)
   __shared__ uint64_t full[kShrinkStages], empty[kShrinkStages], done;
   __shared__ uint32_t tmem_sh;
   __shared__ int issued_sh;
+  __shared__ int2 slab_sh[kShrinkSlabs];
   const int block = blockIdx.x >> 1, half = blockIdx.x & 1;
-  const int s0 = p.blocks[block] + 16 * (int)blockIdx.y;
-  const int ns = min(16, p.blocks[block + 1] - s0);
+  const int s0 = p.blocks[block] + kShrinkSlabs * (int)blockIdx.y;
+  const int ns = min(kShrinkSlabs, p.blocks[block + 1] - s0);
   const int m0 = block * 256 + half * BM;
   if (ns <= 0 || m0 >= p.M) return;  // block-uniform
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -93,6 +95,7 @@ __global__ void __launch_bounds__(128)
     fence_barrier_init();
   }
   if (warp == 0) tmem_alloc(&tmem_sh, tmem_cols);
+  if (tid >= 96 && tid < 96 + ns) slab_sh[tid - 96] = p.slabs[s0 + tid - 96];
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -112,7 +115,7 @@ __global__ void __launch_bounds__(128)
       mbar_expect_tx(&full[st], BM * BK * 2 + ns * 16 * BK * 2);
       tma_load_2d(sx, &mapX, &full[st], kb * BK, m0);
       for (int s = 0; s < ns; ++s) {
-        const int2 sl = p.slabs[s0 + s];
+        const int2 sl = slab_sh[s];
         tma_load_2d(sx + BM * BK * 2 + s * 16 * BK * 2, &mapA, &full[st], kb * BK,
                     sl.x * p.R + 16 * sl.y);
       }
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(128)
   const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
   if (ok) {
     for (int s = 0; s < ns; ++s) {
-      const int2 sl = p.slabs[s0 + s];
+      const int2 sl = slab_sh[s];
       uint32_t r[16];
       tmem_ld16(tmem + lane_off + 16 * s, r);
       tmem_ld_wait();
@@ -226,31 +229,44 @@ __device__ __noinline__ void repair(const GemmLora& p, int64_t row, int n0, floa
 }
 
 // 32 accumulators of a row -> outputs (bias, activation).  Columns past N hold
-// whatever the tile computed there and are not stored.
+// whatever the tile computed there and are not stored.  check: the tile has
+// slabs, so a value that is not finite may not be the row's own.
 __device__ __forceinline__ void finish32(const GemmLora& p, const uint32_t (&r)[32], int64_t row,
-                                         int n0, float (&v)[32]) {
+                                         int n0, bool check, float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-  float t = 0.f;  // stays 0 while every value is finite
-#pragma unroll
-  for (int j = 0; j < 32; ++j) t = fmaf(v[j], 0.f, t);
-  if (t != 0.f && row < p.M) {
-    float again[32];  // a copy, so that v stays in registers
-#pragma unroll
-    for (int j = 0; j < 32; ++j) again[j] = v[j];
-    repair(p, row, n0, again);
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = again[j];
-    return;
-  }
-  if (p.bias) {
+  if (check) {
+    f32x2 t[4];  // stay 0 while every value is finite
 #pragma unroll
     for (int j = 0; j < 32; j += 2)
-      if (n0 + j < p.N) {
-        const float2 b = *reinterpret_cast<const float2*>(p.bias + n0 + j);
+      t[(j >> 1) & 3] = fma2(pk2(v[j], v[j + 1]), splat2(0.f), j < 8 ? splat2(0.f) : t[(j >> 1) & 3]);
+    const float2 t0 = unpk2(t[0]), t1 = unpk2(t[1]), t2 = unpk2(t[2]), t3 = unpk2(t[3]);
+    const float sum = ((t0.x + t0.y) + (t1.x + t1.y)) + ((t2.x + t2.y) + (t3.x + t3.y));
+    if (sum != 0.f && row < p.M) {
+      float again[32];  // a copy, so that v stays in registers
+#pragma unroll
+      for (int j = 0; j < 32; ++j) again[j] = v[j];
+      repair(p, row, n0, again);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = again[j];
+      return;
+    }
+  }
+  if (p.bias) {
+    if (n0 + 32 <= p.N) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n0 + j));
         v[j] += b.x;
         v[j + 1] += b.y;
+        v[j + 2] += b.z;
+        v[j + 3] += b.w;
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (n0 + j < p.N) v[j] += p.bias[n0 + j];
+    }
   }
   if (p.act == ACT_GELU) {
 #pragma unroll
@@ -325,12 +341,24 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool u_ready = false;
+    // a tile's slabs (bounds, and the first 8 of them) are read a tile ahead: read
+    // when they are needed, each costs the ring a trip to memory
+    int s0 = 0, s1 = 0;
+    if (unit < num_tiles) {
+      const int blk = block_of(unit / n_tiles);
+      s0 = p.blocks[blk];
+      s1 = p.blocks[blk + 1];
+    }
     for (int t = unit; t < num_tiles && !abort_sh; t += units) {
       const int mt = t / n_tiles, nb = t % n_tiles;
       const int m0 = mt * F::kTileM + (int)rank * BM;
       const int n0 = nb * BN + (int)rank * F::kBRows;
-      const int blk = block_of(mt);
-      const int s0 = p.blocks[blk], s1 = p.blocks[blk + 1];
+      int2 ahead[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ahead[i] = s0 + i < s1 ? p.slabs[s0 + i] : make_int2(0, 0);
+      const int t2 = t + units < num_tiles ? t + units : t;
+      const int next0 = p.blocks[block_of(t2 / n_tiles)];
+      const int next1 = p.blocks[block_of(t2 / n_tiles) + 1];
       // first row of this CTA's 128 within a slab of U
       const int u_row = PAIR ? (int)rank * BM : (mt & 1) * BM;
       const int steps = k_blocks + (s1 - s0 + SLABS_PER_STAGE - 1) / SLABS_PER_STAGE;
@@ -342,44 +370,39 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
         }
         uint8_t* sa = smem + stage * F::kStageBytes;
         uint8_t* sb = sa + F::kABytes;
-        const int sl0 = s0 + (kb - k_blocks) * SLABS_PER_STAGE;
-        const int ns = kb < k_blocks ? 0 : min(SLABS_PER_STAGE, s1 - sl0);
-        const uint32_t bytes =
-            kb < k_blocks ? F::kStageBytes : ns * (SLAB_A + F::kBRows * 32);
+        const int e = kb - k_blocks;  // which four slabs
+        const int sl0 = s0 + e * SLABS_PER_STAGE;
+        const int ns = e < 0 ? 0 : min(SLABS_PER_STAGE, s1 - sl0);
+        const uint32_t bytes = e < 0 ? F::kStageBytes : ns * (SLAB_A + F::kBRows * 32);
         if (ns > 0 && !u_ready) {
           pdl_wait();
           fence_async_global();
           u_ready = true;
         }
-        if (PAIR) {
-          // both CTAs' bytes are counted on rank 0's barrier
-          const uint32_t bar0 = mapa_shared(smem_u32(&full_bar[stage]), 0);
-          if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * bytes);
-          if (ns == 0) {
-            tma_load_2d_pair(sa, &mapX, bar0, kb * BK, m0);
-            tma_load_2d_pair(sb, &mapW, bar0, kb * BK, n0);
-          }
-          for (int s = 0; s < ns; ++s) {
-            const int2 sl = p.slabs[sl0 + s];
-            tma_load_2d_pair(sa + s * SLAB_A, &mapU, bar0, 0, (sl0 + s) * 256 + u_row);
-            tma_load_2d_pair(sb + s * F::kBRows * 32, &mapB, bar0, 16 * sl.y, sl.x * p.N + n0);
-          }
+        // both CTAs' bytes of a pair are counted on rank 0's barrier
+        const uint32_t bar0 = PAIR ? mapa_shared(smem_u32(&full_bar[stage]), 0) : 0;
+        if (!PAIR || rank == 0) mbar_expect_tx(&full_bar[stage], (PAIR ? 2 : 1) * bytes);
+        auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
+          if (PAIR) tma_load_2d_pair(dst, map, bar0, x, y);
+          else tma_load_2d(dst, map, &full_bar[stage], x, y);
+        };
+        if (e < 0) {
+          load(sa, &mapX, kb * BK, m0);
+          load(sb, &mapW, kb * BK, n0);
         } else {
-          mbar_expect_tx(&full_bar[stage], bytes);
-          if (ns == 0) {
-            tma_load_2d(sa, &mapX, &full_bar[stage], kb * BK, m0);
-            tma_load_2d(sb, &mapW, &full_bar[stage], kb * BK, n0);
-          }
-          for (int s = 0; s < ns; ++s) {
-            const int2 sl = p.slabs[sl0 + s];
-            tma_load_2d(sa + s * SLAB_A, &mapU, &full_bar[stage], 0, (sl0 + s) * 256 + u_row);
-            tma_load_2d(sb + s * F::kBRows * 32, &mapB, &full_bar[stage], 16 * sl.y,
-                        sl.x * p.N + n0);
+#pragma unroll
+          for (int s = 0; s < SLABS_PER_STAGE; ++s) {
+            if (s >= ns) break;
+            const int2 sl = e == 0 ? ahead[s] : e == 1 ? ahead[4 + s] : p.slabs[sl0 + s];
+            load(sa + s * SLAB_A, &mapU, 0, (sl0 + s) * 256 + u_row);
+            load(sb + s * F::kBRows * 32, &mapB, 16 * sl.y, sl.x * p.N + n0);
           }
         }
         ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
+      s0 = next0;
+      s1 = next1;
     }
     if (!u_ready) pdl_wait();  // this kernel's end implies the first one's
     if (!PAIR || rank == 0) {
@@ -393,10 +416,15 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     int stage = 0;
     uint32_t phase = 0;
     int local = 0;
+    auto slabs_of = [&](int t) {
+      const int blk = block_of((t < num_tiles ? t : unit) / n_tiles);
+      return p.blocks[blk + 1] - p.blocks[blk];
+    };
+    int next_slabs = unit < num_tiles ? slabs_of(unit) : 0;  // read a tile ahead
     for (int t = unit; t < num_tiles && !abort_sh; t += units, ++local) {
       const int b = local & 1;
-      const int blk = block_of(t / n_tiles);
-      const int n_slabs = p.blocks[blk + 1] - p.blocks[blk];
+      const int n_slabs = next_slabs;
+      next_slabs = slabs_of(t + units);
       if (!mbar_wait<true>(&tempty_bar[b], ((local >> 1) & 1) ^ 1)) {
         record_err(13);
         abort_sh = 1;
@@ -449,6 +477,8 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     int sbuf = 0, local = 0;
     for (int t = unit; t < num_tiles; t += units, ++local) {
       const int b = local & 1;
+      const int blk = block_of(t / n_tiles);
+      const bool check = p.blocks[blk + 1] > p.blocks[blk];
       const int row0 = (t / n_tiles) * F::kTileM + (int)rank * BM + q * 32;
       const int64_t row = row0 + lane;
       const int col0 = (t % n_tiles) * BN;
@@ -474,7 +504,7 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
             float v[32];
             tmem_ld32(tacc + c + 32 * k2, r);
             tmem_ld_wait();
-            finish32(p, r, row, col0 + c + 32 * k2, v);
+            finish32(p, r, row, col0 + c + 32 * k2, check, v);
             __syncwarp();
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -503,7 +533,7 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
           tmem_ld_wait();
           if (row >= p.M) continue;
           float v[32];
-          finish32(p, r, row, col0 + c, v);
+          finish32(p, r, row, col0 + c, check, v);
           bf16* out = p.C + row * p.ldc + col0 + c;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
@@ -600,10 +630,10 @@ cudaError_t launch_gemm(const GemmLora& p, const bf16* U, cudaStream_t st) {
 }
 
 cudaError_t launch_shrink(const GemmLora& p, bf16* U, cudaStream_t st) {
-  const int slabs = std::min(16, p.max_slabs);
+  const int slabs = std::min(kShrinkSlabs, p.max_slabs);
   const int smem = kShrinkStages * (BM * BK * 2 + slabs * 16 * BK * 2) + 1024;
   static std::atomic<uint64_t> attr_done{0};
-  constexpr int most = kShrinkStages * (BM * BK * 2 + 16 * 16 * BK * 2) + 1024;
+  constexpr int most = kShrinkStages * (BM * BK * 2 + kShrinkSlabs * 16 * BK * 2) + 1024;
   if (cudaError_t rc = ensure_smem_attr(lora_shrink_kernel, most, attr_done)) return rc;
   CUtensorMap mx, ma;
   if (!make_map_bf16(&mx, p.X, p.K, p.M, (uint64_t)p.ldx * 2, BK, BM) ||
@@ -611,7 +641,7 @@ cudaError_t launch_shrink(const GemmLora& p, bf16* U, cudaStream_t st) {
     return cudaErrorInvalidValue;
   uint32_t cols = 32;
   while ((int)cols < 16 * slabs) cols *= 2;
-  const int groups = (p.max_slabs + 15) / 16;
+  const int groups = (p.max_slabs + kShrinkSlabs - 1) / kShrinkSlabs;
   if (groups > 65535) return cudaErrorInvalidConfiguration;
   lora_shrink_kernel<<<dim3(2 * p.n_blocks, groups), 128, smem, st>>>(mx, ma, p, U, slabs, cols);
   return cudaGetLastError();
@@ -623,7 +653,7 @@ cudaError_t launch_shrink(const GemmLora& p, bf16* U, cudaStream_t st) {
 bool gemm_lora_tc_supported(const GemmLora& p) {
   auto on = [](const void* q, int a) { return !(reinterpret_cast<uintptr_t>(q) & (a - 1)); };
   if (p.K < 8 || p.K % 8 || p.N % 8 || p.ldx % 8 || p.ldc % 8) return false;
-  if (!on(p.X, 16) || !on(p.W, 16) || !on(p.C, 16) || !on(p.bias, 8)) return false;
+  if (!on(p.X, 16) || !on(p.W, 16) || !on(p.C, 16) || !on(p.bias, 16)) return false;
   if (p.n_slabs > 0 && (p.R % 8 || !on(p.A, 16) || !on(p.B, 16))) return false;
   return (int64_t)p.n_adapters * p.N <= 0x7fffffff && (int64_t)p.n_adapters * p.R <= 0x7fffffff;
 }
