@@ -251,7 +251,7 @@ typedef struct sj_lora_plan_info {
   int32_t M;         /* rows */
   int32_t rank, n_adapters;
   int32_t n_blocks;  /* blocks of 256 rows */
-  int32_t n_slabs;   /* (block, adapter, 16 of its ranks) */
+  int32_t n_slabs;   /* (block, adapter, 16 of its ranks), in fours */
   int32_t max_slabs; /* of one block */
   int64_t off_blocks, off_slabs; /* word offsets into the plan */
 } sj_lora_plan_info;

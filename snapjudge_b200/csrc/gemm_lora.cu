@@ -141,7 +141,9 @@ int sj_gemm_lora(const sj_gemm_lora_args* a, const sj_lora_plan_info* info, cons
   p.n_slabs = info->n_slabs;
   p.max_slabs = info->max_slabs;
   p.rows = plan;
-  p.blocks = plan + info->off_blocks;
+  p.blocks = reinterpret_cast<const int2*>(plan + info->off_blocks);
+  const int per = (info->rank + 15) / 16;
+  p.unit = per % 4 == 0 ? 4 : per % 2 == 0 ? 2 : 1;
   p.slabs = reinterpret_cast<const int2*>(plan + info->off_slabs);
   const auto st = static_cast<cudaStream_t>(stream);
   const bool tc = sjb::gemm_lora_tc_supported(p) && !(reinterpret_cast<uintptr_t>(workspace) & 15);

@@ -14,11 +14,12 @@ struct GemmLora {
   int M, N, K, R, act, n_adapters;
   int n_blocks, n_slabs, max_slabs;  // max_slabs: of any one block
   const int32_t* rows;    // plan: adapter of each row
-  const int32_t* blocks;  // plan: [n_blocks + 1]
+  const int2* blocks;     // plan: first slab (a multiple of 4) and slabs of each block
   const int2* slabs;      // plan: (adapter, sixteen)
+  int unit;               // slabs that one load of B takes: 4, 2 or 1
 };
 
-// tcgen05 kernels (gemm_lora_tc.cu); U: n_slabs x 256 x 16 bf16 of workspace.
+// tcgen05 kernels (gemm_lora_tc.cu); U: n_slabs / 4 x 256 x 64 bf16 of workspace.
 bool gemm_lora_tc_supported(const GemmLora& p);
 cudaError_t gemm_lora_tc(const GemmLora& p, void* U, cudaStream_t st);
 // As attn_tc_take_status, for these kernels.

@@ -3,7 +3,7 @@
 // Two kernels.  The first computes, for each block of 256 rows and each adapter
 // that a row of the block uses (the plan's slabs, 16 ranks each),
 // U = scale_a X A_a^T, rounded to bf16, with zeros in the rows that do not use
-// the adapter.  The second is a GEMM whose contraction runs over K and then over
+// the adapter; four slabs side by side make rows of 64.  The second is a GEMM whose contraction runs over K and then over
 // the block's slabs: [X | U_1 U_2 ...] [W | B_1 B_2 ...]^T, so the adapters cost
 // one more tcgen05.mma (K = 16) for each slab of a tile and no pass over C.  A
 // row's zeros select its own adapter; 0 x NaN or infinity of another tenant's
@@ -12,9 +12,11 @@
 //
 // GEMM CTA: as gemm_tc.cu (warp 0 loads, warp 1 issues the MMAs, the other
 // warps write tile i while tile i + 1 is computed; TMEM double-buffered), in
-// the forms 256 x 256 by a pair of CTAs, and 128 x BN by one.  A slab is a
-// 128-row (B: BN-row) tile of 32 bytes, 32-byte swizzled; four of them take the
-// place of one 64-wide k-block in the ring of stages.  The second kernel is
+// the forms 256 x 256 by a pair of CTAs, and 128 x BN by one.  Four slabs take the
+// place of one 64-wide k-block in the ring of stages: their U is one load, their B
+// one to four (`unit` slabs of one adapter at a time, rows of 32, 64 or 128 bytes,
+// swizzled over as many).  With a load of 32-byte rows for each slab of U as well,
+// the slabs cost the loads as much as whole k-blocks.  The second kernel is
 // launched while the first runs (programmatic dependent launch) and waits for
 // it before its first slab, after all of a tile's k-blocks are on their way.
 // Bounded waits and wind-down as in gemm_tc.cu.
@@ -35,19 +37,19 @@ namespace {
 using namespace tc;
 
 constexpr int BM = 128, BK = 64;
-constexpr int SLAB_A = BM * 32;  // bytes of a slab of U for 128 rows
 constexpr int SLABS_PER_STAGE = 4;
 
 __device__ __forceinline__ void record_err(int code) { atomicCAS(&g_gemm_lora_err, 0, code); }
 
-// K-major tile of 16 bf16 (32 bytes) a row, 32-byte swizzle: 8-row groups 256 bytes apart
-__device__ __forceinline__ uint64_t desc_kmajor_sw32(uint32_t addr) {
+// K-major tile of `unit` x 16 bf16 a row, swizzled over the row's 32, 64 or 128
+// bytes: 8-row groups that many times 8 bytes apart
+__device__ __forceinline__ uint64_t desc_unit(uint32_t addr, int unit) {
   uint64_t d = 0;
   d |= (uint64_t)((addr >> 4) & 0x3FFF);
   d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(256 >> 4) << 32;
+  d |= (uint64_t)(unit * 256 >> 4) << 32;
   d |= (uint64_t)1 << 46;
-  d |= (uint64_t)6 << 61;
+  d |= (uint64_t)(unit == 4 ? 2 : unit == 2 ? 4 : 6) << 61;
   return d;
 }
 __device__ __forceinline__ void pdl_launch_dependents() {
@@ -77,8 +79,9 @@ __global__ void __launch_bounds__(128)
   __shared__ int issued_sh;
   __shared__ int2 slab_sh[kShrinkSlabs];
   const int block = blockIdx.x >> 1, half = blockIdx.x & 1;
-  const int s0 = p.blocks[block] + kShrinkSlabs * (int)blockIdx.y;
-  const int ns = min(kShrinkSlabs, p.blocks[block + 1] - s0);
+  const int2 mine_of = p.blocks[block];
+  const int s0 = mine_of.x + kShrinkSlabs * (int)blockIdx.y;
+  const int ns = min(kShrinkSlabs, mine_of.y - kShrinkSlabs * (int)blockIdx.y);
   const int m0 = block * 256 + half * BM;
   if (ns <= 0 || m0 >= p.M) return;  // block-uniform
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(128)
       uint8_t* sx = smem + st * stage_bytes;
       mbar_expect_tx(&full[st], BM * BK * 2 + ns * 16 * BK * 2);
       tma_load_2d(sx, &mapX, &full[st], kb * BK, m0);
-      for (int s = 0; s < ns; ++s) {
+      for (int s = 0; s < ns; s += p.unit) {
         const int2 sl = slab_sh[s];
         tma_load_2d(sx + BM * BK * 2 + s * 16 * BK * 2, &mapA, &full[st], kb * BK,
                     sl.x * p.R + 16 * sl.y);
@@ -168,7 +171,8 @@ __global__ void __launch_bounds__(128)
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         w[e] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      uint4* u = reinterpret_cast<uint4*>(U + ((int64_t)(s0 + s) * 256 + half * BM + tid) * 16);
+      uint4* u = reinterpret_cast<uint4*>(
+          U + ((int64_t)((s0 + s) >> 2) * 256 + half * BM + tid) * 64 + ((s0 + s) & 3) * 16);
       u[0] = make_uint4(w[0], w[1], w[2], w[3]);
       u[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
@@ -343,66 +347,65 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     bool u_ready = false;
     // a tile's slabs (bounds, and the first 8 of them) are read a tile ahead: read
     // when they are needed, each costs the ring a trip to memory
-    int s0 = 0, s1 = 0;
-    if (unit < num_tiles) {
-      const int blk = block_of(unit / n_tiles);
-      s0 = p.blocks[blk];
-      s1 = p.blocks[blk + 1];
-    }
+    const int us = p.unit;
+    int2 blk = unit < num_tiles ? p.blocks[block_of(unit / n_tiles)] : make_int2(0, 0);
     for (int t = unit; t < num_tiles && !abort_sh; t += units) {
       const int mt = t / n_tiles, nb = t % n_tiles;
       const int m0 = mt * F::kTileM + (int)rank * BM;
       const int n0 = nb * BN + (int)rank * F::kBRows;
+      const int s0 = blk.x, s1 = blk.x + blk.y;
       int2 ahead[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) ahead[i] = s0 + i < s1 ? p.slabs[s0 + i] : make_int2(0, 0);
-      const int t2 = t + units < num_tiles ? t + units : t;
-      const int next0 = p.blocks[block_of(t2 / n_tiles)];
-      const int next1 = p.blocks[block_of(t2 / n_tiles) + 1];
+      const int2 next = p.blocks[block_of((t + units < num_tiles ? t + units : t) / n_tiles)];
       // first row of this CTA's 128 within a slab of U
       const int u_row = PAIR ? (int)rank * BM : (mt & 1) * BM;
-      const int steps = k_blocks + (s1 - s0 + SLABS_PER_STAGE - 1) / SLABS_PER_STAGE;
-      for (int kb = 0; kb < steps; ++kb) {
+      // a stage's barrier (both CTAs' bytes of a pair are counted on rank 0's)
+      auto open_stage = [&](uint32_t bytes) -> bool {
         if (!mbar_wait<true>(&empty_bar[stage], phase ^ 1)) {
           record_err(11);
           abort_sh = 1;
-          break;
+          return false;
         }
+        if (!PAIR || rank == 0) mbar_expect_tx(&full_bar[stage], (PAIR ? 2 : 1) * bytes);
+        return true;
+      };
+      auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
+        if (PAIR) tma_load_2d_pair(dst, map, mapa_shared(smem_u32(&full_bar[stage]), 0), x, y);
+        else tma_load_2d(dst, map, &full_bar[stage], x, y);
+      };
+      auto next_stage = [&]() {
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      };
+      bool ok = true;
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!(ok = open_stage(F::kStageBytes))) break;
         uint8_t* sa = smem + stage * F::kStageBytes;
-        uint8_t* sb = sa + F::kABytes;
-        const int e = kb - k_blocks;  // which four slabs
-        const int sl0 = s0 + e * SLABS_PER_STAGE;
-        const int ns = e < 0 ? 0 : min(SLABS_PER_STAGE, s1 - sl0);
-        const uint32_t bytes = e < 0 ? F::kStageBytes : ns * (SLAB_A + F::kBRows * 32);
-        if (ns > 0 && !u_ready) {
+        load(sa, &mapX, kb * BK, m0);
+        load(sa + F::kABytes, &mapW, kb * BK, n0);
+        next_stage();
+      }
+      for (int e = 0; ok && e * SLABS_PER_STAGE < s1 - s0; ++e) {
+        const int sl0 = s0 + e * SLABS_PER_STAGE, ns = min(SLABS_PER_STAGE, s1 - sl0);
+        if (!u_ready) {
           pdl_wait();
           fence_async_global();
           u_ready = true;
         }
-        // both CTAs' bytes of a pair are counted on rank 0's barrier
-        const uint32_t bar0 = PAIR ? mapa_shared(smem_u32(&full_bar[stage]), 0) : 0;
-        if (!PAIR || rank == 0) mbar_expect_tx(&full_bar[stage], (PAIR ? 2 : 1) * bytes);
-        auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
-          if (PAIR) tma_load_2d_pair(dst, map, bar0, x, y);
-          else tma_load_2d(dst, map, &full_bar[stage], x, y);
-        };
-        if (e < 0) {
-          load(sa, &mapX, kb * BK, m0);
-          load(sb, &mapW, kb * BK, n0);
-        } else {
+        if (!(ok = open_stage(F::kABytes + (ns + us - 1) / us * us * F::kBRows * 32))) break;
+        uint8_t* sa = smem + stage * F::kStageBytes;
+        uint8_t* sb = sa + F::kABytes;
+        load(sa, &mapU, 0, (sl0 >> 2) * 256 + u_row);
 #pragma unroll
-          for (int s = 0; s < SLABS_PER_STAGE; ++s) {
-            if (s >= ns) break;
-            const int2 sl = e == 0 ? ahead[s] : e == 1 ? ahead[4 + s] : p.slabs[sl0 + s];
-            load(sa + s * SLAB_A, &mapU, 0, (sl0 + s) * 256 + u_row);
-            load(sb + s * F::kBRows * 32, &mapB, 16 * sl.y, sl.x * p.N + n0);
-          }
+        for (int s = 0; s < SLABS_PER_STAGE; ++s) {
+          if (s >= ns || s % us) continue;
+          const int2 sl = e == 0 ? ahead[s] : e == 1 ? ahead[4 + s] : p.slabs[sl0 + s];
+          load(sb + s * F::kBRows * 32, &mapB, 16 * sl.y, sl.x * p.N + n0);
         }
-        ++issued;
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        next_stage();
       }
-      s0 = next0;
-      s1 = next1;
+      blk = next;
     }
     if (!u_ready) pdl_wait();  // this kernel's end implies the first one's
     if (!PAIR || rank == 0) {
@@ -417,8 +420,7 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     uint32_t phase = 0;
     int local = 0;
     auto slabs_of = [&](int t) {
-      const int blk = block_of((t < num_tiles ? t : unit) / n_tiles);
-      return p.blocks[blk + 1] - p.blocks[blk];
+      return p.blocks[block_of((t < num_tiles ? t : unit) / n_tiles)].y;
     };
     int next_slabs = unit < num_tiles ? slabs_of(unit) : 0;  // read a tile ahead
     for (int t = unit; t < num_tiles && !abort_sh; t += units, ++local) {
@@ -432,36 +434,47 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
       }
       fence_after_sync();
       const uint32_t d = tmem_base + b * BN;
-      const int steps = k_blocks + (n_slabs + SLABS_PER_STAGE - 1) / SLABS_PER_STAGE;
-      for (int kb = 0; kb < steps; ++kb) {
+      bool ok = true;
+      auto open_stage = [&]() -> bool {
         if (!mbar_wait<true>(&full_bar[stage], phase)) {
           record_err(14);
           abort_sh = 1;
-          break;
+          return false;
         }
         fence_after_sync();
-        const uint32_t a_addr = smem_u32(smem + stage * F::kStageBytes);
-        const uint32_t b_addr = a_addr + F::kABytes;
-        if (kb < k_blocks) {
-#pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            const uint64_t ad = desc_kmajor_sw128(a_addr + kk * 32);
-            const uint64_t bd = desc_kmajor_sw128(b_addr + kk * 32);
-            if (PAIR) mma_bf16_pair(d, ad, bd, IDESC, (kb | kk) != 0);
-            else mma_bf16(d, ad, bd, IDESC, (kb | kk) != 0);
-          }
-        } else {
-          const int ns = min(SLABS_PER_STAGE, n_slabs - (kb - k_blocks) * SLABS_PER_STAGE);
-          for (int s = 0; s < ns; ++s) {
-            const uint64_t ad = desc_kmajor_sw32(a_addr + s * SLAB_A);
-            const uint64_t bd = desc_kmajor_sw32(b_addr + s * F::kBRows * 32);
-            if (PAIR) mma_bf16_pair(d, ad, bd, IDESC, 1u);
-            else mma_bf16(d, ad, bd, IDESC, 1u);
-          }
-        }
+        return true;
+      };
+      auto close_stage = [&]() {
         if (PAIR) mma_commit_pair(&empty_bar[stage], 0x3);
         else mma_commit(&empty_bar[stage]);
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      };
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!(ok = open_stage())) break;
+        const uint32_t a_addr = smem_u32(smem + stage * F::kStageBytes);
+        const uint32_t b_addr = a_addr + F::kABytes;
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {
+          const uint64_t ad = desc_kmajor_sw128(a_addr + kk * 32);
+          const uint64_t bd = desc_kmajor_sw128(b_addr + kk * 32);
+          if (PAIR) mma_bf16_pair(d, ad, bd, IDESC, (kb | kk) != 0);
+          else mma_bf16(d, ad, bd, IDESC, (kb | kk) != 0);
+        }
+        close_stage();
+      }
+      for (int s0 = 0; ok && s0 < n_slabs; s0 += SLABS_PER_STAGE) {
+        if (!(ok = open_stage())) break;
+        const uint32_t a_addr = smem_u32(smem + stage * F::kStageBytes);
+        const uint32_t b_addr = a_addr + F::kABytes;
+        const int ns = min(SLABS_PER_STAGE, n_slabs - s0);
+        for (int s = 0; s < ns; ++s) {
+          const uint64_t ad = desc_kmajor_sw128(a_addr + s * 32);
+          const uint64_t bd = desc_unit(
+              b_addr + s / p.unit * p.unit * F::kBRows * 32 + s % p.unit * 32, p.unit);
+          if (PAIR) mma_bf16_pair(d, ad, bd, IDESC, 1u);
+          else mma_bf16(d, ad, bd, IDESC, 1u);
+        }
+        close_stage();
       }
       if (PAIR) mma_commit_pair(&tfull_bar[b], 0x3);
       else mma_commit(&tfull_bar[b]);
@@ -477,8 +490,7 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     int sbuf = 0, local = 0;
     for (int t = unit; t < num_tiles; t += units, ++local) {
       const int b = local & 1;
-      const int blk = block_of(t / n_tiles);
-      const bool check = p.blocks[blk + 1] > p.blocks[blk];
+      const bool check = p.blocks[block_of(t / n_tiles)].y > 0;
       const int row0 = (t / n_tiles) * F::kTileM + (int)rank * BM + q * 32;
       const int64_t row = row0 + lane;
       const int col0 = (t % n_tiles) * BN;
@@ -570,18 +582,21 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
   }
 }
 
-// 2-D map of rows of 16 bf16 (32 bytes), 32-byte swizzle
-bool make_map_slab(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows,
-                   uint64_t row_bytes, uint32_t box_rows) {
+// 2-D map of B: boxes of `unit` x 16 ranks, swizzled over the box's row
+bool make_map_ranks(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, int unit,
+                    uint32_t box_rows) {
   auto fn = encode_fn();
-  if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || (row_bytes & 15)) return false;
+  if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || inner * 2 % 16) return false;
   cuuint64_t dims[2] = {inner, rows};
-  cuuint64_t strides[1] = {row_bytes};
-  cuuint32_t box[2] = {16, box_rows};
+  cuuint64_t strides[1] = {inner * 2};
+  cuuint32_t box[2] = {16u * (uint32_t)unit, box_rows};
   cuuint32_t es[2] = {1, 1};
+  const CUtensorMapSwizzle swizzle = unit == 4   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : unit == 2 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                 : CU_TENSOR_MAP_SWIZZLE_32B;
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int BN, bool PAIR>
@@ -597,9 +612,8 @@ cudaError_t launch_gemm(const GemmLora& p, const bf16* U, cudaStream_t st) {
     return cudaErrorInvalidValue;
   if (p.n_slabs == 0) {
     mu = mb = mx;  // never read
-  } else if (!make_map_slab(&mu, U, 16, (uint64_t)p.n_slabs * 256, 32, BM) ||
-             !make_map_slab(&mb, p.B, p.R, (uint64_t)p.n_adapters * p.N, (uint64_t)p.R * 2,
-                            F::kBRows)) {
+  } else if (!make_map_bf16(&mu, U, 64, (uint64_t)p.n_slabs / 4 * 256, 128, 64, BM) ||
+             !make_map_ranks(&mb, p.B, p.R, (uint64_t)p.n_adapters * p.N, p.unit, F::kBRows)) {
     return cudaErrorInvalidValue;
   }
   const int n_tiles = (p.N + BN - 1) / BN;
@@ -637,7 +651,8 @@ cudaError_t launch_shrink(const GemmLora& p, bf16* U, cudaStream_t st) {
   if (cudaError_t rc = ensure_smem_attr(lora_shrink_kernel, most, attr_done)) return rc;
   CUtensorMap mx, ma;
   if (!make_map_bf16(&mx, p.X, p.K, p.M, (uint64_t)p.ldx * 2, BK, BM) ||
-      !make_map_bf16(&ma, p.A, p.K, (uint64_t)p.n_adapters * p.R, (uint64_t)p.K * 2, BK, 16))
+      !make_map_bf16(&ma, p.A, p.K, (uint64_t)p.n_adapters * p.R, (uint64_t)p.K * 2, BK,
+                     16 * p.unit))
     return cudaErrorInvalidValue;
   uint32_t cols = 32;
   while ((int)cols < 16 * slabs) cols *= 2;

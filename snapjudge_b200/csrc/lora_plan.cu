@@ -2,9 +2,11 @@
 //
 // The plan holds
 //   rows    the adapter of each row (-1: none);
-//   blocks  for each block of 256 rows, the first of its slabs, and their end;
+//   blocks  2 words for each block of 256 rows: the first of its slabs, a multiple
+//           of 4, and how many it has;
 //   slabs   2 words each: an adapter that a row of the block uses, and which
-//           16 of its ranks (adapters in the order of their first row).
+//           16 of its ranks (adapters in the order of their first row); filled up
+//           to a multiple of 4 in each block.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -34,11 +36,12 @@ int make_plan(const int32_t* cu, int B, const int32_t* ids, int n_adapters, int 
   const int M = cu[B];
   const int per = (rank + 15) / 16;
   const int nb = (int)(((long long)M + 255) / 256);
-  std::vector<int32_t> slabs, first((size_t)nb + 1, 0);
+  std::vector<int32_t> slabs, blocks((size_t)nb * 2, 0);
   std::vector<int> seen((size_t)n_adapters, -1);  // last block that listed the adapter
   int32_t most = 0;
   for (int k = 0, b = 0; k < nb; ++k) {
     const int r1 = std::min<long long>(M, 256ll * (k + 1));
+    blocks[2 * k] = (int32_t)(slabs.size() / 2);
     while (b > 0 && cu[b] > 256 * k) --b;
     for (; b < B && cu[b] < r1; ++b) {
       if (cu[b + 1] <= 256 * k || cu[b + 1] == cu[b]) continue;
@@ -50,9 +53,10 @@ int make_plan(const int32_t* cu, int B, const int32_t* ids, int n_adapters, int 
         slabs.push_back(s);
       }
     }
-    if (slabs.size() / 2 > 0x7fffff) return bad("the batch needs too many adapter blocks");
-    first[k + 1] = (int32_t)(slabs.size() / 2);
-    most = std::max(most, first[k + 1] - first[k]);
+    if (slabs.size() / 2 > 0x7ffff0) return bad("the batch needs too many adapter blocks");
+    blocks[2 * k + 1] = (int32_t)(slabs.size() / 2) - blocks[2 * k];
+    most = std::max(most, blocks[2 * k + 1]);
+    slabs.resize((slabs.size() + 7) / 8 * 8, 0);
   }
   info->M = M;
   info->rank = rank;
@@ -61,13 +65,13 @@ int make_plan(const int32_t* cu, int B, const int32_t* ids, int n_adapters, int 
   info->n_slabs = (int32_t)(slabs.size() / 2);
   info->max_slabs = most;
   info->off_blocks = ((long long)M + 3) / 4 * 4;
-  info->off_slabs = info->off_blocks + ((long long)nb + 1 + 3) / 4 * 4;
+  info->off_slabs = info->off_blocks + (2ll * nb + 3) / 4 * 4;
   info->plan_len = info->off_slabs + (long long)slabs.size();
   if (!plan) return SJ_OK;
   if (plan_len < info->plan_len) return bad("the plan's memory is too small");
   std::fill(plan, plan + info->plan_len, 0);
   for (int b = 0; b < B; ++b) std::fill(plan + cu[b], plan + cu[b + 1], ids[b]);
-  std::copy(first.begin(), first.end(), plan + info->off_blocks);
+  std::copy(blocks.begin(), blocks.end(), plan + info->off_blocks);
   std::copy(slabs.begin(), slabs.end(), plan + info->off_slabs);
   return SJ_OK;
 }

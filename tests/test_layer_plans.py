@@ -197,14 +197,20 @@ def test_lora_plan_lists_each_blocks_adapters(cu, ids, n, rank):
     assert rc == 0
     rows = np.repeat(np.asarray(ids, int), np.diff(cu))
     assert info.M == len(rows) and (plan[:info.M] == rows).all()
-    first = plan[info.off_blocks:info.off_blocks + info.n_blocks + 1]
+    blocks = plan[info.off_blocks:info.off_blocks + 2 * info.n_blocks].reshape(-1, 2)
     slabs = plan[info.off_slabs:info.off_slabs + 2 * info.n_slabs].reshape(-1, 2)
-    assert info.n_blocks == -(-info.M // 256) and first[0] == 0 and first[-1] == info.n_slabs
-    for k in range(info.n_blocks):
+    assert info.n_blocks == -(-info.M // 256)
+    assert info.max_slabs == max(blocks[:, 1], default=0)
+    at = 0
+    for k, (first, count) in enumerate(blocks):
+        assert first == at and first % 4 == 0
+        at += -(-count // 4) * 4
         want = {(a, s) for a in set(rows[256 * k:256 * k + 256].tolist()) - {-1}
                 for s in range(-(-rank // 16))}
-        mine = [tuple(x) for x in slabs[first[k]:first[k + 1]].tolist()]
+        mine = [tuple(x) for x in slabs[first:first + count].tolist()]
         assert len(mine) == len(want) and set(mine) == want
+        assert [s for _, s in mine] == list(range(-(-rank // 16))) * (len(mine) // -(-rank // 16))
+    assert at == info.n_slabs
 
 
 @pytest.mark.parametrize("cu,ids,n,rank,word", [
