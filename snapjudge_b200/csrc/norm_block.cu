@@ -13,13 +13,19 @@
 // pitches and the addresses allow it, else 1.  Rows too wide for that are read
 // once per statistic instead (norm_block_wide).
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "../../include/snapjudge_b200.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "tc_host.h"
 
 namespace sjb {
 namespace {
+
+// norm_block_rows: widest row and its weights' memory (112 KB: two blocks an SM)
+constexpr int kRowsMost = 5600, kRowsSmem = 5 * (kRowsMost + 6) / 4 * 4 * 4;
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]);
@@ -62,7 +68,8 @@ __device__ __forceinline__ void store_vec<bf16, 4>(bf16* p, const float (&v)[4])
   *reinterpret_cast<uint2*>(p) = u;
 }
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+// relative error about 2^-21; 0 and 1 at the ends
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 
 // The segment that owns row r (largest b with cu[b] <= r), by a whole warp: 32
 // probes a step instead of a binary search's chain of dependent loads.
@@ -92,7 +99,7 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
 }
 
 template <typename TX, typename TR, typename TY, int VEC, int NC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 1024)
+__global__ void __launch_bounds__(WARP ? 128 : VEC == 1 ? 512 : 1024)
     norm_block_kernel(const sj_norm_block_args p) {
   __shared__ float red[4][32];
   const int lane = threadIdx.x & 31;
@@ -197,6 +204,195 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
   }
 }
 
+// The same for rows that start anywhere: their pitches are alike modulo 4 elements,
+// so row r's x, r, x', y (and row gate) all start (r * pitch) mod 4 elements into a
+// 16-byte group, and groups of 4 are loaded and stored whole except at the row's
+// ends.  A block keeps to rows of one such shift (`classes` of them: 1, 2 or 4) and
+// holds the weights in shared memory moved by it, for all its rows.
+template <typename TX, typename TR, typename TY, int NC, bool WARP>
+__global__ void __launch_bounds__(256) norm_block_rows(const __grid_constant__ sj_norm_block_args p,
+                                                       int classes) {
+  extern __shared__ __align__(16) float wsh[];
+  __shared__ float red[2][4][8];
+  const int lane = threadIdx.x & 31;
+  const int G = WARP ? 32 : (int)blockDim.x;
+  const int t = WARP ? lane : (int)threadIdx.x;
+  const int cls = (int)(blockIdx.x % classes);
+  const int sft = (int)((cls * p.ldx) & 3);
+  const int nch = (p.D + sft + 3) / 4, pitch = (p.D + 3 + 3) / 4 * 4;
+  const float inv_d = 1.f / (float)p.D;
+  // weights by place in the shifted row: post_w, post_b, channel gate, pre_w, pre_b
+  const float* src[5] = {p.post_w, p.post_b,
+                         p.gate_mode == SJ_GATE_CHANNEL ? static_cast<const float*>(p.gate) : nullptr,
+                         p.pre_w, p.pre_b};
+  float* at[5];
+  int held = 0;
+#pragma unroll
+  for (int a = 0; a < 5; ++a) {
+    at[a] = wsh + held * pitch;
+    if (!src[a]) continue;
+    ++held;
+    for (int j = threadIdx.x; j < pitch; j += blockDim.x)
+      at[a][j] = j >= sft && j - sft < p.D ? src[a][j - sft] : 0.f;
+  }
+  __syncthreads();
+
+  // Groups wholly inside the row are loaded and stored as they are; the others (the
+  // row's ends, and past them: NC is the least that holds a row, so they are a
+  // thread's first or one of its last two) load some whole group and are put right
+  // afterwards.  Which they are does not depend on the row.
+  bool whole[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int k = t + G * c;
+    whole[c] = (c > 0 && c < NC - 2) || (4 * k >= sft && 4 * k + 4 <= p.D + sft);
+  }
+  auto inside = [&](int j) { return j >= sft && j < p.D + sft; };
+  auto at_ends = [&](auto&& f) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if ((c == 0 || c >= NC - 2) && !whole[c]) f(c, t + G * c);
+  };
+  const int64_t per_block = WARP ? blockDim.x / 32 : 1;
+  const int64_t step = (int64_t)(gridDim.x / classes) * per_block;
+  int64_t i = (int64_t)(blockIdx.x / classes) * per_block + (WARP ? threadIdx.x / 32 : 0);
+  for (int par = 0; cls + classes * i < p.M; i += step, par ^= 1) {
+    const int64_t row = cls + classes * i;
+    const TX* x = static_cast<const TX*>(p.x) + row * p.ldx - sft;
+    const TR* r = static_cast<const TR*>(p.r) + row * p.ldr - sft;
+    float xv[NC][4], zv[NC][4];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int k = t + G * c, kk = whole[c] ? k : 1;
+      load_vec<TX, 4>(x + 4 * kk, xv[c]);
+      load_vec<TR, 4>(r + 4 * kk, zv[c]);
+    }
+    at_ends([&](int c, int k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = inside(4 * k + e);
+        xv[c][e] = in ? io<TX>::ld(x + 4 * k + e) : 0.f;
+        zv[c][e] = in ? io<TR>::ld(r + 4 * k + e) : 0.f;
+      }
+    });
+    int seg = 0;
+    if (p.gate_mode == SJ_GATE_SEGMENT) seg = warp_seg_of_row(p.cu_seqlens, p.n_segs, row, lane);
+    auto normalise = [&](float (&v)[NC][4], float* red_mean, float* red_var) {
+      float mean = 0.f;
+      if (p.kind == SJ_NORM_LN) {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s += (v[c][0] + v[c][1]) + (v[c][2] + v[c][3]);
+        mean = group_sum<WARP>(s, red_mean) * inv_d;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[c][e] -= mean;
+        at_ends([&](int c, int k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[c][e] = inside(4 * k + e) ? v[c][e] : 0.f;
+        });
+      }
+      float q = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        q += (v[c][0] * v[c][0] + v[c][1] * v[c][1]) + (v[c][2] * v[c][2] + v[c][3] * v[c][3]);
+      const float inv = rsqrtf(group_sum<WARP>(q, red_var) * inv_d + p.eps);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c][e] *= inv;
+    };
+    // v <- v w (+ b), also where v is outside the row
+    auto affine = [&](float (&v)[NC][4], int w, bool bias) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int k = c < NC - 1 ? t + G * c : min(t + G * c, nch - 1);
+        float u[4];
+        load_vec<float, 4>(at[w] + 4 * k, u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c][e] *= u[e];
+        if (bias) {
+          load_vec<float, 4>(at[w + 1] + 4 * k, u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[c][e] += u[e];
+        }
+      }
+    };
+    auto store = [&](auto* out, const float (&v)[NC][4]) {
+      using T = std::remove_pointer_t<decltype(out)>;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int k = t + G * c;
+        if (whole[c]) store_vec<T, 4>(out + 4 * k, v[c]);
+      }
+      at_ends([&](int c, int k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (inside(4 * k + e)) out[4 * k + e] = io<T>::cvt(v[c][e]);
+      });
+    };
+    auto row_gate = [&](auto* base) {
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(base)>>;
+      const T* gr = base + row * p.ldg - sft;
+      float g[NC][4];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int k = t + G * c;
+        load_vec<T, 4>(gr + 4 * (whole[c] ? k : 1), g[c]);
+      }
+      at_ends([&](int c, int k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[c][e] = inside(4 * k + e) ? io<T>::ld(gr + 4 * k + e) : 0.f;
+      });
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) zv[c][e] *= sigmoid(g[c][e]);
+    };
+    if (p.post_w) {
+      normalise(zv, red[par][0], red[par][1]);
+      affine(zv, 0, p.post_b != nullptr);
+    }
+    if (p.gate_mode == SJ_GATE_CHANNEL) {
+      affine(zv, 2, false);
+    } else if (p.gate_mode == SJ_GATE_SEGMENT) {  // a segment's gate starts where it may
+      const float* gs = static_cast<const float*>(p.gate) + (int64_t)seg * p.D - sft;
+      float g[NC][4];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int k = t + G * c, kk = whole[c] ? k : 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[c][e] = __ldg(gs + 4 * kk + e);
+      }
+      at_ends([&](int c, int k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[c][e] = inside(4 * k + e) ? __ldg(gs + 4 * k + e) : 0.f;
+      });
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) zv[c][e] *= g[c][e];
+    } else if (p.gate_mode == SJ_GATE_ROW) {
+      if (p.gate_type == SJ_TYPE_BF16) row_gate(static_cast<const bf16*>(p.gate));
+      else row_gate(static_cast<const float*>(p.gate));
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) xv[c][e] = p.alpha * xv[c][e] + p.beta * zv[c][e];
+    store(static_cast<TX*>(p.x_out) + row * p.ldxo - sft, xv);
+    if (!p.y) continue;
+    at_ends([&](int c, int k) {  // nothing outside the row in its statistics
+#pragma unroll
+      for (int e = 0; e < 4; ++e) xv[c][e] = inside(4 * k + e) ? xv[c][e] : 0.f;
+    });
+    normalise(xv, red[par][2], red[par][3]);
+    affine(xv, 3, p.pre_b != nullptr);
+    store(static_cast<TY*>(p.y) + row * p.ldy - sft, xv);
+  }
+}
+
 // Rows wider than the registers of a block: every statistic reads the row again.
 template <typename TX, typename TR, typename TY>
 __global__ void __launch_bounds__(1024) norm_block_wide(const sj_norm_block_args p) {
@@ -264,11 +460,56 @@ cudaError_t launch(const sj_norm_block_args& a, int group, cudaStream_t st) {
     kernel<<<(unsigned)blocks, threads, 0, st>>>(a);
     return cudaGetLastError();
   };
-  if (nc <= 2) return go(norm_block_kernel<TX, TR, TY, VEC, 2, WARP>);
-  if (nc <= 4) return go(norm_block_kernel<TX, TR, TY, VEC, 4, WARP>);
-  if constexpr (WARP || VEC == 1) {  // blocks take at most 4 chunks of 4 (dispatch)
-    if (nc <= 6) return go(norm_block_kernel<TX, TR, TY, VEC, 6, WARP>);
-    if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, VEC, 8, WARP>);
+  if constexpr (VEC == 4) {
+    if (nc <= 2) return go(norm_block_kernel<TX, TR, TY, 4, 2, WARP>);
+    if (nc <= 4) return go(norm_block_kernel<TX, TR, TY, 4, 4, WARP>);
+    if constexpr (WARP) {  // blocks take at most 4 chunks of 4 (dispatch)
+      if (nc <= 6) return go(norm_block_kernel<TX, TR, TY, 4, 6, WARP>);
+      if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, 4, 8, WARP>);
+    }
+  } else {
+    if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, 1, 8, WARP>);
+    if (nc <= 16) return go(norm_block_kernel<TX, TR, TY, 1, 16, WARP>);
+    if constexpr (WARP) {
+      if (nc <= 24) return go(norm_block_kernel<TX, TR, TY, 1, 24, WARP>);
+      if (nc <= 32) return go(norm_block_kernel<TX, TR, TY, 1, 32, WARP>);
+    }
+  }
+  return cudaErrorInvalidConfiguration;
+}
+
+template <typename TX, typename TR, typename TY, bool WARP>
+cudaError_t launch_rows(const sj_norm_block_args& a, int group, cudaStream_t st) {
+  // the widest shift's groups
+  const int nc = ((a.D + (a.ldx % 2 ? 3 : a.ldx % 4 ? 2 : 0) + 3) / 4 + group - 1) / group;
+  const int classes = a.ldx % 4 == 0 ? 1 : a.ldx % 2 == 0 ? 2 : 4;
+  // short rows: smaller blocks and more of them (60,000 x 1001: 131 against 146 us
+  // with 256 threads; 200,000 x 301: 197 against 252 us with 128)
+  const int threads = !WARP ? group : nc > 4 ? 256 : 128;
+  const int held = (a.post_w != nullptr) + (a.post_b != nullptr) + (a.pre_w != nullptr) +
+                   (a.pre_b != nullptr) + (a.gate_mode == SJ_GATE_CHANNEL);
+  const int smem = held * ((a.D + 6) / 4 * 4) * 4;
+  const int rows = WARP ? threads / 32 : 1;  // of a block at a time
+  const int64_t units = (a.M + rows - 1) / rows;
+  const int64_t most = (int64_t)tc::sm_count() * (WARP ? (nc > 4 ? 4 : 16) : 1024 / threads);
+  const unsigned blocks = (unsigned)((std::min(most, units) + classes - 1) / classes * classes);
+  auto go = [&](auto count) -> cudaError_t {  // instantiated once for each NC
+    constexpr int NC = decltype(count)::value;
+    static std::atomic<uint64_t> attr_done{0};  // per device ordinal
+    auto kernel = norm_block_rows<TX, TR, TY, NC, WARP>;
+    if (cudaError_t rc = tc::ensure_smem_attr(kernel, kRowsSmem, attr_done)) return rc;
+    kernel<<<blocks, threads, smem, st>>>(a, classes);
+    return cudaGetLastError();
+  };
+  switch (nc) {
+    case 1: return go(std::integral_constant<int, 1>{});
+    case 2: return go(std::integral_constant<int, 2>{});
+    case 3: return go(std::integral_constant<int, 3>{});
+    case 4: return go(std::integral_constant<int, 4>{});
+    case 5: return go(std::integral_constant<int, 5>{});
+    case 6: return go(std::integral_constant<int, 6>{});
+    case 7: return go(std::integral_constant<int, 7>{});
+    case 8: return go(std::integral_constant<int, 8>{});
   }
   return cudaErrorInvalidConfiguration;
 }
@@ -285,15 +526,25 @@ cudaError_t dispatch(const sj_norm_block_args& a, cudaStream_t st) {
                     on(a.x, a.x_type) && on(a.x_out, a.x_type) && on(a.r, a.r_type) &&
                     on(a.y, a.y_type) && on(a.post_w, 0) && on(a.post_b, 0) && on(a.pre_w, 0) &&
                     on(a.pre_b, 0) && on(a.gate, row_gate ? a.gate_type : 0);
-  const int chunks = vec4 ? a.D / 4 : a.D;
-  if (chunks <= 32 * 8) {
-    return vec4 ? launch<TX, TR, TY, 4, true>(a, 32, st) : launch<TX, TR, TY, 1, true>(a, 32, st);
+  // whole vectors inside rows that start anywhere, alike in every tensor
+  const bool alike = a.ldxo % 4 == a.ldx % 4 && a.ldr % 4 == a.ldx % 4 &&
+                     (!a.y || a.ldy % 4 == a.ldx % 4) && (!row_gate || a.ldg % 4 == a.ldx % 4) &&
+                     on(a.x, a.x_type) && on(a.x_out, a.x_type) && on(a.r, a.r_type) &&
+                     on(a.y, a.y_type) && (!row_gate || on(a.gate, a.gate_type));
+  if (alike && !vec4 && a.D >= 8 && a.D <= kRowsMost) {
+    if (a.D <= 1024 - 3) return launch_rows<TX, TR, TY, true>(a, 32, st);
+    return launch_rows<TX, TR, TY, false>(a, a.D <= 2048 - 3 ? 64 : a.D <= 4096 - 3 ? 128 : 256, st);
   }
-  int group = 64;
-  while (group < 1024 && chunks > 4 * group) group *= 2;
-  if (chunks <= 4 * group || (!vec4 && chunks <= 8 * group))
-    return vec4 ? launch<TX, TR, TY, 4, false>(a, group, st)
-                : launch<TX, TR, TY, 1, false>(a, group, st);
+  if (vec4) {
+    const int chunks = a.D / 4;
+    if (chunks <= 32 * 8) return launch<TX, TR, TY, 4, true>(a, 32, st);
+    for (int group = 64; group <= 1024; group *= 2)
+      if (chunks <= 4 * group) return launch<TX, TR, TY, 4, false>(a, group, st);
+  } else {
+    if (a.D <= 32 * 32) return launch<TX, TR, TY, 1, true>(a, 32, st);
+    for (int group = 64; group <= 512; group *= 2)
+      if (a.D <= 16 * group) return launch<TX, TR, TY, 1, false>(a, group, st);
+  }
   if (a.M > 0x7fffffff) return cudaErrorInvalidConfiguration;
   norm_block_wide<TX, TR, TY><<<(unsigned)a.M, 1024, 0, st>>>(a);
   return cudaGetLastError();

@@ -505,7 +505,10 @@ def check_norm(M, D, kind="ln", post=True, bias=False, mode=None, xt=F32, rt=BF,
 
 
 @pytest.mark.parametrize("M,D", [(1, 768), (37, 768), (300, 1024), (65, 64), (9, 100), (7, 1),
-                                 (12, 3), (50, 257), (33, 1001), (20, 1536), (9, 2048), (5, 4095),
+                                 (12, 3), (30, 7), (30, 9), (31, 130), (50, 257), (50, 385),
+                                 (33, 510), (33, 641), (33, 774), (33, 899), (33, 1001), (40, 1021),
+                                 (40, 1023), (20, 1536), (20, 2043), (9, 2048), (9, 2047),
+                                 (5, 4093), (5, 4095), (6, 5599), (6, 5601),
                                  (3, 8192), (3, 16384), (2, 9001), (2, 20000)])
 @pytest.mark.parametrize("kind,bias", [("ln", True), ("rms", False)])
 def test_norm_block_widths(M, D, kind, bias):
