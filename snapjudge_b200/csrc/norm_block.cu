@@ -98,7 +98,8 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
   return warp_sum(lane < nw ? red[lane] : 0.f);
 }
 
-template <typename TX, typename TR, typename TY, int VEC, int NC, bool WARP>
+// ROWGATE: the gate is [M, D]; read with x and r.
+template <typename TX, typename TR, typename TY, int VEC, int NC, bool WARP, bool ROWGATE>
 __global__ void __launch_bounds__(WARP ? 128 : VEC == 1 ? 512 : 1024)
     norm_block_kernel(const sj_norm_block_args p) {
   __shared__ float red[4][32];
@@ -113,7 +114,8 @@ __global__ void __launch_bounds__(WARP ? 128 : VEC == 1 ? 512 : 1024)
   const int nch = (p.D + VEC - 1) / VEC;  // VEC divides D
   const float inv_d = 1.f / (float)p.D;
 
-  float xv[NC][VEC], zv[NC][VEC];
+  float xv[NC][VEC], zv[NC][VEC], gv[ROWGATE ? NC : 1][VEC];
+  const int64_t g0 = row * p.ldg;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int k = t + G * c;
@@ -122,6 +124,12 @@ __global__ void __launch_bounds__(WARP ? 128 : VEC == 1 ? 512 : 1024)
     if (k < nch) {
       load_vec<TX, VEC>(x + VEC * k, xv[c]);
       load_vec<TR, VEC>(r + VEC * k, zv[c]);
+      if constexpr (ROWGATE) {
+        if (p.gate_type == SJ_TYPE_BF16)
+          load_vec<bf16, VEC>(static_cast<const bf16*>(p.gate) + g0 + VEC * k, gv[c]);
+        else
+          load_vec<float, VEC>(static_cast<const float*>(p.gate) + g0 + VEC * k, gv[c]);
+      }
     }
   }
   int seg = 0;
@@ -173,18 +181,12 @@ __global__ void __launch_bounds__(WARP ? 128 : VEC == 1 ? 512 : 1024)
     const int k = t + G * c;
     if (k >= nch) continue;
     if (p.post_w) affine(zv[c], k, p.post_w, p.post_b);
-    if (p.gate_mode != SJ_GATE_NONE) {
-      float g[VEC];
-      if (p.gate_mode == SJ_GATE_ROW) {
-        if (p.gate_type == SJ_TYPE_BF16)
-          load_vec<bf16, VEC>(static_cast<const bf16*>(p.gate) + row * p.ldg + VEC * k, g);
-        else
-          load_vec<float, VEC>(static_cast<const float*>(p.gate) + row * p.ldg + VEC * k, g);
+    if constexpr (ROWGATE) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = sigmoid(g[e]);
-      } else {
-        load_vec<float, VEC>(static_cast<const float*>(p.gate) + (int64_t)seg * p.D + VEC * k, g);
-      }
+      for (int e = 0; e < VEC; ++e) zv[c][e] *= sigmoid(gv[c][e]);
+    } else if (p.gate_mode != SJ_GATE_NONE) {
+      float g[VEC];
+      load_vec<float, VEC>(static_cast<const float*>(p.gate) + (int64_t)seg * p.D + VEC * k, g);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) zv[c][e] *= g[e];
     }
@@ -460,22 +462,25 @@ cudaError_t launch(const sj_norm_block_args& a, int group, cudaStream_t st) {
     kernel<<<(unsigned)blocks, threads, 0, st>>>(a);
     return cudaGetLastError();
   };
-  if constexpr (VEC == 4) {
-    if (nc <= 2) return go(norm_block_kernel<TX, TR, TY, 4, 2, WARP>);
-    if (nc <= 4) return go(norm_block_kernel<TX, TR, TY, 4, 4, WARP>);
-    if constexpr (WARP) {  // blocks take at most 4 chunks of 4 (dispatch)
-      if (nc <= 6) return go(norm_block_kernel<TX, TR, TY, 4, 6, WARP>);
-      if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, 4, 8, WARP>);
+  auto pick = [&](auto rg) -> cudaError_t {
+    constexpr bool RG = decltype(rg)::value;
+    if constexpr (VEC == 4) {
+      if (nc <= 2) return go(norm_block_kernel<TX, TR, TY, 4, 2, WARP, RG>);
+      if (nc <= 4) return go(norm_block_kernel<TX, TR, TY, 4, 4, WARP, RG>);
+      if constexpr (WARP) {  // blocks take at most 4 chunks of 4 (dispatch)
+        if (nc <= 6) return go(norm_block_kernel<TX, TR, TY, 4, 6, WARP, RG>);
+        if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, 4, 8, WARP, RG>);
+      }
+    } else {
+      if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, 1, 8, WARP, RG>);
+      if (nc <= 16) return go(norm_block_kernel<TX, TR, TY, 1, 16, WARP, RG>);
+      if constexpr (WARP) {
+        if (nc <= 32) return go(norm_block_kernel<TX, TR, TY, 1, 32, WARP, RG>);
+      }
     }
-  } else {
-    if (nc <= 8) return go(norm_block_kernel<TX, TR, TY, 1, 8, WARP>);
-    if (nc <= 16) return go(norm_block_kernel<TX, TR, TY, 1, 16, WARP>);
-    if constexpr (WARP) {
-      if (nc <= 24) return go(norm_block_kernel<TX, TR, TY, 1, 24, WARP>);
-      if (nc <= 32) return go(norm_block_kernel<TX, TR, TY, 1, 32, WARP>);
-    }
-  }
-  return cudaErrorInvalidConfiguration;
+    return cudaErrorInvalidConfiguration;
+  };
+  return a.gate_mode == SJ_GATE_ROW ? pick(std::true_type{}) : pick(std::false_type{});
 }
 
 template <typename TX, typename TR, typename TY, bool WARP>
@@ -537,9 +542,13 @@ cudaError_t dispatch(const sj_norm_block_args& a, cudaStream_t st) {
   }
   if (vec4) {
     const int chunks = a.D / 4;
-    if (chunks <= 32 * 8) return launch<TX, TR, TY, 4, true>(a, 32, st);
+    // a warp holds up to 8 groups a lane (with a gate for each row, a third array,
+    // 4: 65,536 x 1024 160 against 282 us); in a block's rows two a thread, so that
+    // more warps share the loads (20,000 x 4096: 191 against 220 us with four)
+    if (chunks <= 32 * (row_gate ? 4 : 8)) return launch<TX, TR, TY, 4, true>(a, 32, st);
     for (int group = 64; group <= 1024; group *= 2)
-      if (chunks <= 4 * group) return launch<TX, TR, TY, 4, false>(a, group, st);
+      if (chunks <= (group < 1024 ? 2 : 4) * group)
+        return launch<TX, TR, TY, 4, false>(a, group, st);
   } else {
     if (a.D <= 32 * 32) return launch<TX, TR, TY, 1, true>(a, 32, st);
     for (int group = 64; group <= 512; group *= 2)
