@@ -274,6 +274,9 @@ typedef struct sj_gemm_lora_args {
   int act;
 } sj_gemm_lora_args;
 
+/* Bytes of device workspace that sj_gemm_lora needs (16-byte aligned; the
+ * caller's, one for each call in flight; the same for every N and K); -1 for a
+ * bad shape. */
 int64_t sj_gemm_lora_workspace(const sj_lora_plan_info* info, int N, int K);
 
 int sj_gemm_lora(const sj_gemm_lora_args* args, const sj_lora_plan_info* info,

@@ -63,6 +63,20 @@ __device__ __forceinline__ void fence_async_global() {
   asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
+// sum of 8 products of bf16
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
+  float s = 0.f;
+  const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&aw[i]));
+    const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&bw[i]));
+    s = fmaf(x.x, y.x, s);
+    s = fmaf(x.y, y.y, s);
+  }
+  return s;
+}
+
 // ---- U = scale_a X A_a^T -------------------------------------------------------
 // One CTA: 128 rows, up to 8 slabs (N = 128); 96 KB of stages, so that two share
 // an SM.  Thread 0 loads, thread 32 issues the MMAs, all four warps write U
@@ -185,7 +199,44 @@ __global__ void __launch_bounds__(128)
   }
 }
 
+// ---- U by rows, for blocks of many adapters: one warp a row -----------------------
+// U[row, r] = scale_a X[row] . A_a[r], rounded to bf16
+__global__ void __launch_bounds__(256)
+    lora_shrink_rows_kernel(const __grid_constant__ GemmLora p, bf16* __restrict__ U) {
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= p.M) return;
+  const int a = p.rows[row];
+  if (a < 0) return;  // its U is not read
+  const float f = p.scale ? p.scale[a] : 1.f;
+  const bf16* x = p.X + row * p.ldx;
+  const bf16* ar = p.A + (int64_t)a * p.R * p.K;
+  for (int r0 = 0; r0 < p.R; r0 += 8) {  // R is a multiple of 8
+    float acc[8] = {};
+    for (int k = 8 * lane; k < p.K; k += 256) {  // and K
+      const uint4 xv = *reinterpret_cast<const uint4*>(x + k);
+      uint4 av[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        av[r] = *reinterpret_cast<const uint4*>(ar + (int64_t)(r0 + r) * p.K + k);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) acc[r] += dot8(xv, av[r]);
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float t = warp_sum(acc[r]);
+      mine = lane == r ? t : mine;
+    }
+    if (lane < 8) U[row * p.R + r0 + lane] = __float2bfloat16(f * mine);
+  }
+}
+
 // ---- the GEMM -----------------------------------------------------------------------
+// GATHER: no slabs; the epilogue adds U[row] . B_a[n], its own adapter's alone, from
+// memory.  For tiles of few columns whose rows use many adapters: 600 rows with 64
+// adapters of rank 8, 768 x 768: 58 slabs in a block.
 template <int BN, bool PAIR>
 struct Cfg {
   static constexpr int kEpiWarps = BN >= 64 ? 8 : 4;
@@ -285,14 +336,31 @@ __device__ __forceinline__ void finish32(const GemmLora& p, const uint32_t (&r)[
   }
 }
 
-template <int BN, bool PAIR>
+// r[j] += U[row] . B_a[n0 + j] for the row's own adapter
+__device__ __forceinline__ void add_own(const GemmLora& p, const bf16* U, int64_t row, int n0,
+                                        uint32_t (&r)[32]) {
+  const int a = p.rows[row];
+  if (a < 0) return;
+  const bf16* b = p.B + ((int64_t)a * p.N + n0) * p.R;
+  for (int r0 = 0; r0 < p.R; r0 += 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(U + row * p.R + r0);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n0 + j < p.N)
+        r[j] = __float_as_uint(
+            __uint_as_float(r[j]) +
+            dot8(u, __ldg(reinterpret_cast<const uint4*>(b + (int64_t)j * p.R + r0))));
+  }
+}
+
+template <int BN, bool PAIR, bool GATHER>
 __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     gemm_lora_kernel(const __grid_constant__ CUtensorMap mapX,
                      const __grid_constant__ CUtensorMap mapW,
                      const __grid_constant__ CUtensorMap mapU,
                      const __grid_constant__ CUtensorMap mapB,
                      const __grid_constant__ CUtensorMap mapC, const __grid_constant__ GemmLora p,
-                     int n_tiles) {
+                     int n_tiles, const bf16* __restrict__ U) {
   using F = Cfg<BN, PAIR>;
   constexpr int STAGES = F::kStages;
   constexpr uint32_t IDESC = idesc_bf16(F::kTileM, BN, false, false);
@@ -353,7 +421,7 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
       const int mt = t / n_tiles, nb = t % n_tiles;
       const int m0 = mt * F::kTileM + (int)rank * BM;
       const int n0 = nb * BN + (int)rank * F::kBRows;
-      const int s0 = blk.x, s1 = blk.x + blk.y;
+      const int s0 = blk.x, s1 = GATHER ? blk.x : blk.x + blk.y;
       int2 ahead[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) ahead[i] = s0 + i < s1 ? p.slabs[s0 + i] : make_int2(0, 0);
@@ -420,7 +488,7 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     uint32_t phase = 0;
     int local = 0;
     auto slabs_of = [&](int t) {
-      return p.blocks[block_of((t < num_tiles ? t : unit) / n_tiles)].y;
+      return GATHER ? 0 : p.blocks[block_of((t < num_tiles ? t : unit) / n_tiles)].y;
     };
     int next_slabs = unit < num_tiles ? slabs_of(unit) : 0;  // read a tile ahead
     for (int t = unit; t < num_tiles && !abort_sh; t += units, ++local) {
@@ -485,12 +553,13 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
     constexpr int PARTS = F::kEpiWarps / 4;  // warps of a row quarter share its columns
+    if constexpr (GATHER) pdl_wait();        // U, read by the epilogue
     const int q = warp & 3, hf = (warp - 2) >> 2;
     uint8_t* stg = smem + STAGES * F::kStageBytes + (warp - 2) * 2 * 32 * 128;
     int sbuf = 0, local = 0;
     for (int t = unit; t < num_tiles; t += units, ++local) {
       const int b = local & 1;
-      const bool check = p.blocks[block_of(t / n_tiles)].y > 0;
+      const bool check = !GATHER && p.blocks[block_of(t / n_tiles)].y > 0;
       const int row0 = (t / n_tiles) * F::kTileM + (int)rank * BM + q * 32;
       const int64_t row = row0 + lane;
       const int col0 = (t % n_tiles) * BN;
@@ -544,6 +613,7 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
           tmem_ld32(tacc + c, r);
           tmem_ld_wait();
           if (row >= p.M) continue;
+          if constexpr (GATHER) add_own(p, U, row, col0 + c, r);
           float v[32];
           finish32(p, r, row, col0 + c, check, v);
           bf16* out = p.C + row * p.ldc + col0 + c;
@@ -599,23 +669,20 @@ bool make_map_ranks(CUtensorMap* m, const void* base, uint64_t inner, uint64_t r
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool PAIR>
-cudaError_t launch_gemm(const GemmLora& p, const bf16* U, cudaStream_t st) {
+template <int BN, bool PAIR, bool GATHER = false>
+cudaError_t launch_gemm(const GemmLora& p, const CUtensorMap& mx, const bf16* U, cudaStream_t st) {
   using F = Cfg<BN, PAIR>;
   static std::atomic<uint64_t> attr_done{0};  // per device ordinal
-  auto kernel = gemm_lora_kernel<BN, PAIR>;
+  auto kernel = gemm_lora_kernel<BN, PAIR, GATHER>;
   if (cudaError_t rc = ensure_smem_attr(kernel, F::kSmem, attr_done)) return rc;
-  CUtensorMap mx, mw, mu, mb, mc;
-  if (!make_map_bf16(&mx, p.X, p.K, p.M, (uint64_t)p.ldx * 2, BK, BM) ||
-      !make_map_bf16(&mw, p.W, p.K, p.N, (uint64_t)p.K * 2, BK, F::kBRows) ||
-      !make_map_bf16(&mc, p.C, p.N, p.M, (uint64_t)p.ldc * 2, 64, 32))
+  CUtensorMap mw, mu = mx, mb = mx, mc = mx;  // those that are not made are not read
+  if (!make_map_bf16(&mw, p.W, p.K, p.N, (uint64_t)p.K * 2, BK, F::kBRows)) return cudaErrorInvalidValue;
+  if (F::kStaged && !make_map_bf16(&mc, p.C, p.N, p.M, (uint64_t)p.ldc * 2, 64, 32))
     return cudaErrorInvalidValue;
-  if (p.n_slabs == 0) {
-    mu = mb = mx;  // never read
-  } else if (!make_map_bf16(&mu, U, 64, (uint64_t)p.n_slabs / 4 * 256, 128, 64, BM) ||
-             !make_map_ranks(&mb, p.B, p.R, (uint64_t)p.n_adapters * p.N, p.unit, F::kBRows)) {
+  if (!GATHER && p.n_slabs > 0 &&
+      (!make_map_bf16(&mu, U, 64, (uint64_t)p.n_slabs / 4 * 256, 128, 64, BM) ||
+       !make_map_ranks(&mb, p.B, p.R, (uint64_t)p.n_adapters * p.N, p.unit, F::kBRows)))
     return cudaErrorInvalidValue;
-  }
   const int n_tiles = (p.N + BN - 1) / BN;
   const int64_t tiles = ((int64_t)p.M + F::kTileM - 1) / F::kTileM * n_tiles;
   if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;
@@ -640,18 +707,17 @@ cudaError_t launch_gemm(const GemmLora& p, const bf16* U, cudaStream_t st) {
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, mu, mb, mc, p, n_tiles);
+  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, mu, mb, mc, p, n_tiles, U);
 }
 
-cudaError_t launch_shrink(const GemmLora& p, bf16* U, cudaStream_t st) {
+cudaError_t launch_shrink(const GemmLora& p, const CUtensorMap& mx, bf16* U, cudaStream_t st) {
   const int slabs = std::min(kShrinkSlabs, p.max_slabs);
   const int smem = kShrinkStages * (BM * BK * 2 + slabs * 16 * BK * 2) + 1024;
   static std::atomic<uint64_t> attr_done{0};
   constexpr int most = kShrinkStages * (BM * BK * 2 + kShrinkSlabs * 16 * BK * 2) + 1024;
   if (cudaError_t rc = ensure_smem_attr(lora_shrink_kernel, most, attr_done)) return rc;
-  CUtensorMap mx, ma;
-  if (!make_map_bf16(&mx, p.X, p.K, p.M, (uint64_t)p.ldx * 2, BK, BM) ||
-      !make_map_bf16(&ma, p.A, p.K, (uint64_t)p.n_adapters * p.R, (uint64_t)p.K * 2, BK,
+  CUtensorMap ma;
+  if (!make_map_bf16(&ma, p.A, p.K, (uint64_t)p.n_adapters * p.R, (uint64_t)p.K * 2, BK,
                      16 * p.unit))
     return cudaErrorInvalidValue;
   uint32_t cols = 32;
@@ -675,15 +741,34 @@ bool gemm_lora_tc_supported(const GemmLora& p) {
 
 cudaError_t gemm_lora_tc(const GemmLora& p, void* U, cudaStream_t st) {
   bf16* u = static_cast<bf16*>(U);
-  if (p.n_slabs > 0)
-    if (cudaError_t rc = launch_shrink(p, u, st)) return rc;
-  if (p.M >= 2048) return launch_gemm<256, true>(p, u, st);
+  CUtensorMap mx;
+  if (!make_map_bf16(&mx, p.X, p.K, p.M, (uint64_t)p.ldx * 2, BK, BM)) return cudaErrorInvalidValue;
   const int64_t mt = (p.M + BM - 1) / BM;
   const int sms = sm_count();
-  if (mt * ((p.N + 255) / 256) >= sms) return launch_gemm<256, false>(p, u, st);
-  if (mt * ((p.N + 127) / 128) >= sms) return launch_gemm<128, false>(p, u, st);
-  if (mt * ((p.N + 63) / 64) >= sms) return launch_gemm<64, false>(p, u, st);
-  return launch_gemm<32, false>(p, u, st);
+  const bool pair = p.M >= 2048;
+  const int bn = pair                                   ? 256
+                 : mt * ((p.N + 255) / 256) >= sms      ? 256
+                 : mt * ((p.N + 127) / 128) >= sms      ? 128
+                 : mt * ((p.N + 63) / 64) >= sms        ? 64
+                                                        : 32;
+  // tiles of few columns pay about 100 cycles for each slab, and 4 x rank for each
+  // column of the gather
+  const bool gather = bn <= 64 && 10 * p.max_slabs > 13 * p.R;
+  if (gather) {
+    lora_shrink_rows_kernel<<<(unsigned)((p.M + 7) / 8), 256, 0, st>>>(p, u);
+    if (cudaError_t rc = cudaGetLastError()) return rc;
+    return bn == 64 ? launch_gemm<64, false, true>(p, mx, u, st)
+                    : launch_gemm<32, false, true>(p, mx, u, st);
+  }
+  if (p.n_slabs > 0)
+    if (cudaError_t rc = launch_shrink(p, mx, u, st)) return rc;
+  if (pair) return launch_gemm<256, true>(p, mx, u, st);
+  switch (bn) {
+    case 256: return launch_gemm<256, false>(p, mx, u, st);
+    case 128: return launch_gemm<128, false>(p, mx, u, st);
+    case 64: return launch_gemm<64, false>(p, mx, u, st);
+    default: return launch_gemm<32, false>(p, mx, u, st);
+  }
 }
 
 cudaError_t gemm_lora_take_status(int* code) {

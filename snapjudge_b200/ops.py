@@ -315,6 +315,7 @@ class LoraPlan:
         check(L.sj_lora_plan(*a, buf.ctypes.data, len(buf), C.byref(self.info)))
         self.info_ref = C.byref(self.info)
         self.n_rows, self.rank, self.n_adapters = self.info.M, rank, n_adapters
+        self.workspace = L.sj_gemm_lora_workspace(self.info_ref, 0, 0)  # of any width
         self.data = _plan_on_device(buf, device)
         self.device = self.data.get_device()
 
@@ -336,7 +337,7 @@ def gemm_lora(X, W, A, B, plan, *, scale=None, bias=None, act=0):
     s = _vec(scale, "scale", (plan.n_adapters,), dev)
     bias_ = _vec(bias, "bias", (N,), dev)
     L = _lib.lib()
-    need = L.sj_gemm_lora_workspace(plan.info_ref, N, K)
+    need = plan.workspace
     C_ = torch.empty((M, N), dtype=torch.bfloat16, device=X.device)
     ws = torch.empty(need, dtype=torch.uint8, device=X.device) if need else None
     args = _gemm_lora_args(X.data_ptr(), w, a, b, s, bias_, C_.data_ptr(), ldx, N, N, K, act)
