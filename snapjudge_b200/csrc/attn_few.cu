@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_few_kernel(const __grid_cons
   const int64_t rest = unit / p.Hkv;
   const int mt = (int)(rest % mtiles);
   const int64_t part = rest / mtiles;
+  // the join's blocks may start now; they wait for this kernel's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (part >= p.n_parts) return;
   const int4 pa = p.parts[2 * part], pb = p.parts[2 * part + 1];
   const int row0 = pa.x, nrows = pa.y, tile0 = pa.z, ntiles = pa.w, ws_row = pb.x;
@@ -300,6 +302,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_few_join(const __grid_consta
   if (grp >= p.n_splits) return;
   const int4 g = p.splits[grp];  // first row, rows, parts, first workspace row
   if (r >= g.y) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int E = DH / 32;
   // lane k takes part k's maximum and sum (32 parts at a time), then every lane
   // adds its dimensions over the parts: no load waits for another part's
@@ -353,8 +356,16 @@ cudaError_t launch(const AttnMasked& p, float* ws, cudaStream_t st) {
   if (p.n_splits == 0) return cudaSuccess;
   const int64_t jb = ((int64_t)p.n_splits * 16 * p.H + kWarps - 1) / kWarps;
   if (jb > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  attn_few_join<DH><<<(unsigned)jb, 32 * kWarps, 0, st>>>(p, ws);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)jb, 1, 1);
+  cfg.blockDim = dim3(32 * kWarps, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_few_join<DH>, p, static_cast<const float*>(ws));
 }
 
 }  // namespace

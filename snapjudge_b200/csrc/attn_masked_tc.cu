@@ -286,13 +286,18 @@ __global__ void __launch_bounds__(kThreads, Shape<DH>::kCtas)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool leader = tid == 0, loader = tid == 96;
   const int group = p.H / p.Hkv;
-  const int cnt =
-      n_work > (int)blockIdx.x ? (n_work - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  // This block's items, longest first: rounds of one item for each block, every
+  // other round in reverse, so that what a block gains in one it pays in the next
+  // (in the same order each time, the first blocks' sums grow).
+  const int V = (int)gridDim.x, v = (int)blockIdx.x;
+  auto work_of = [&](int k) { return k * V + (k & 1 ? V - 1 - v : v); };
+  const int rounds = n_work / V;
+  const int cnt = rounds + (work_of(rounds) < n_work);
 
   auto decode_chunk = [&](int c) {
     const int k = c * CHUNK + tid;
     if (tid < CHUNK && k < cnt) {
-      const int w = (int)blockIdx.x + k * (int)gridDim.x;
+      const int w = work_of(k);
       const int4 v = p.items[w / p.H];
       Item it;
       it.row0 = v.x;
