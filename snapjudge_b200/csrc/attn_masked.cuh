@@ -16,7 +16,7 @@ struct AttnMasked {
   const float* rel_bias;      // [H, 2 rel_max + 1] or null
   int rel_max;
   const float* slopes;        // [H] or null
-  int n_rows, n_keys, n_items;
+  int n_rows, n_keys, n_items, n_tiles;
   bool rows_consecutive;      // query row r is key row r (no q_rows)
   const int4* rows;           // plan: 2 x int4 for each query row
   const int4* items;          // plan: one for each query tile
@@ -50,6 +50,7 @@ inline AttnMasked attn_masked_params(const sj_attn_masked_args& a, const sj_attn
   p.n_rows = info.n_rows;
   p.n_keys = info.n_keys;
   p.n_items = info.n_items;
+  p.n_tiles = info.n_tiles;
   p.rows_consecutive = info.n_rows == info.n_keys;
   p.rows = reinterpret_cast<const int4*>(plan);
   p.items = reinterpret_cast<const int4*>(plan + info.off_items);

@@ -28,6 +28,8 @@
 // A masked key has p = 0, and 0 x NaN or infinity of its V would still reach
 // the row: a row whose output is not finite is computed again over its visible
 // keys alone (attn_masked_row).
+// At head_dim 128 neither an S buffer for odd tiles (MMAs beside the softmax: 155
+// against 143 us) nor two threads for a row (146) paid.
 // Waits are bounded and failures carried to the next block-wide barrier, as in
 // attn_tc.cu.
 #include <string.h>
@@ -713,7 +715,13 @@ cudaError_t launch(const AttnMasked& p, cudaStream_t st) {
     return cudaErrorInvalidValue;
   const int64_t work = (int64_t)p.n_items * p.H;
   if (work > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  const int grid = (int)std::min<int64_t>(work, (int64_t)F::kCtas * sm_count());
+  // Long items (10 key tiles on average) go to a block each, in order as blocks end,
+  // which evens out what they differ by: 12 ragged causal segments, head_dim 128, 114
+  // against 144 us.  Short ones (7: 425 against 369 us) are worth a list for each
+  // resident block, whose next item's loads start before the last one ends.
+  const int grid = p.n_tiles >= 10ll * p.n_items
+                       ? (int)work
+                       : (int)std::min<int64_t>(work, (int64_t)F::kCtas * sm_count());
   kernel<<<grid, kThreads, F::kSmem, st>>>(mq, mk, mv, p, make_score(p), (int)work);
   return cudaGetLastError();
 }
