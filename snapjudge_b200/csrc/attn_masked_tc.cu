@@ -19,8 +19,9 @@
 // one CTA with P in columns of its own, so that MMAs overlap the softmax, 554 and
 // 1,341; two chains with warps of their own for loads, MMAs and work lists, 748
 // and 1,218: fewer softmax warps cost more than the overlap gains.
-// The reference maximum moves only when a tile's maximum exceeds it by 2^8; the
-// row's O in TMEM and its sum are then rescaled.  Sums and O are fp32; P is
+// The reference maximum moves only when a tile's maximum exceeds it by 2^32 (bf16 and
+// fp32 hold such P and sums as exactly as small ones); the row's O in TMEM and its sum
+// are then rescaled.  Sums and O are fp32; P is
 // rounded to bf16 because V is bf16 and the MMA takes one type.
 // Table biases of consecutive query rows: the 191 distances of a (query, key)
 // tile pair are staged in shared memory one tile ahead; the row reads entry
@@ -58,7 +59,7 @@ constexpr int KV_STAGES = 2;
 template <bool CAP>
 constexpr int poly_pairs() { return CAP ? 0 : 1; }
 constexpr int CHUNK = 32;  // work items decoded at a time
-constexpr float kRescaleLog2 = 8.f;
+constexpr float kRescaleLog2 = 32.f;
 constexpr float kLog2e = 1.4426950408889634f;
 // Staged distances: 191 used.  Two copies, the second one entry ahead, so that
 // a row's pair of columns is one aligned 8-byte load whatever the row; the

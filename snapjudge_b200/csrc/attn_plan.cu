@@ -22,6 +22,7 @@
 //   few     the groups' key tiles, as above.
 #include <algorithm>
 #include <array>
+#include <cstdlib>
 #include <new>
 #include <vector>
 
@@ -147,6 +148,11 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
     const int r1 = std::min(nr, r0 + 128);
     Item it{r0, r1 - r0, (int)tiles.size(), 0};
     cover(rows.data(), r0, r1, iv, tiles);
+    // nearest first: where scores fall with the distance, the maximum is found at once
+    const int mid = rows[(r0 + r1) / 2].pos;
+    auto away = [&](int e) { return std::abs((e < 0 ? ~e : e) + 32 - mid); };
+    std::stable_sort(tiles.begin() + it.tile0, tiles.end(),
+                     [&](int x, int y) { return away(x) < away(y); });
     if (tiles.size() > 0x7fffffff) return bad("the batch needs too many key tiles");
     it.tiles = (int)tiles.size() - it.tile0;
     items.push_back(it);
