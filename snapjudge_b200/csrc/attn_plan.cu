@@ -51,8 +51,9 @@ void cover(const Row* rows, int r0, int r1, std::vector<Iv>& iv, std::vector<int
   Iv ca{0, 0x7fffffff}, cb{0, 0x7fffffff};  // keys that every row sees, by its intervals
   for (int r = r0; r < r1; ++r) {
     const Row& w = rows[r];
-    if (w.a1 > w.a0) iv.push_back({w.a0, w.a1});
-    if (w.b1 > w.b0) iv.push_back({w.b0, w.b1});
+    // (neighbours mostly have the same intervals)
+    if (w.a1 > w.a0 && (r == r0 || w.a0 != rows[r - 1].a0 || w.a1 != rows[r - 1].a1)) iv.push_back({w.a0, w.a1});
+    if (w.b1 > w.b0 && (r == r0 || w.b0 != rows[r - 1].b0 || w.b1 != rows[r - 1].b1)) iv.push_back({w.b0, w.b1});
     ca.a = std::max(ca.a, w.a0), ca.b = std::min(ca.b, w.a1);
     cb.a = std::max(cb.a, w.b0), cb.b = std::min(cb.b, w.b1);
   }
@@ -192,6 +193,7 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
     }
   }
 
+  if (few.size() > 0x7fffffff || ws_rows > 0x7fffffff) return bad("the batch needs too many key tiles");
   info->n_rows = nr;
   info->n_keys = T;
   info->n_items = (int)items.size();

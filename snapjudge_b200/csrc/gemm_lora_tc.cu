@@ -557,9 +557,14 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
     const int q = warp & 3, hf = (warp - 2) >> 2;
     uint8_t* stg = smem + STAGES * F::kStageBytes + (warp - 2) * 2 * 32 * 128;
     int sbuf = 0, local = 0;
+    auto slabs_of = [&](int t) {
+      return GATHER || t >= num_tiles ? 0 : p.blocks[block_of(t / n_tiles)].y;
+    };
+    int next_slabs = slabs_of(unit);  // read a tile ahead
     for (int t = unit; t < num_tiles; t += units, ++local) {
       const int b = local & 1;
-      const bool check = !GATHER && p.blocks[block_of(t / n_tiles)].y > 0;
+      const bool check = next_slabs > 0;
+      next_slabs = slabs_of(t + units);
       const int row0 = (t / n_tiles) * F::kTileM + (int)rank * BM + q * 32;
       const int64_t row = row0 + lane;
       const int col0 = (t % n_tiles) * BN;

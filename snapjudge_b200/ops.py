@@ -235,9 +235,16 @@ class AttnPlan:
                                  int(causal), int(window), _FORMS[form])
         self.info = _lib.AttnPlanInfo()
         L = _lib.lib()
-        check(L.sj_attn_plan(C.byref(args), None, 0, C.byref(self.info)))
-        buf = np.empty(max(1, self.info.plan_len), np.int32)
-        check(L.sj_attn_plan(C.byref(args), buf.ctypes.data, len(buf), C.byref(self.info)))
+        # a plan of most batches fits the first guess; one that does not says its size
+        rows = int(cu[-1]) if q_rows is None else len(q_rows)
+        buf = np.empty(12 * max(rows, 0) + 4096, np.int32)
+        self.info.plan_len = 0
+        rc = L.sj_attn_plan(C.byref(args), buf.ctypes.data, len(buf), C.byref(self.info))
+        if rc and self.info.plan_len > len(buf):
+            buf = np.empty(self.info.plan_len, np.int32)
+            rc = L.sj_attn_plan(C.byref(args), buf.ctypes.data, len(buf), C.byref(self.info))
+        check(rc)
+        buf = buf[:max(1, self.info.plan_len)]
         self.info_ref = C.byref(self.info)
         self.n_rows, self.n_keys = self.info.n_rows, self.info.n_keys
         self.data = _plan_on_device(buf, device)
@@ -310,9 +317,14 @@ class LoraPlan:
         self.info = _lib.LoraPlanInfo()
         L = _lib.lib()
         a = (cu.ctypes.data, len(ids), ids.ctypes.data, n_adapters, rank)
-        check(L.sj_lora_plan(*a, None, 0, C.byref(self.info)))
-        buf = np.empty(max(1, self.info.plan_len), np.int32)
-        check(L.sj_lora_plan(*a, buf.ctypes.data, len(buf), C.byref(self.info)))
+        buf = np.empty(2 * max(int(cu[-1]), 0) + 4096, np.int32)
+        self.info.plan_len = 0
+        rc = L.sj_lora_plan(*a, buf.ctypes.data, len(buf), C.byref(self.info))
+        if rc and self.info.plan_len > len(buf):
+            buf = np.empty(self.info.plan_len, np.int32)
+            rc = L.sj_lora_plan(*a, buf.ctypes.data, len(buf), C.byref(self.info))
+        check(rc)
+        buf = buf[:max(1, self.info.plan_len)]
         self.info_ref = C.byref(self.info)
         self.n_rows, self.rank, self.n_adapters = self.info.M, rank, n_adapters
         self.workspace = L.sj_gemm_lora_workspace(self.info_ref, 0, 0)  # of any width
