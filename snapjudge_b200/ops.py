@@ -153,7 +153,7 @@ def _at(t):
 def _here(t, name):
     """t's CUDA device, which has to be the current one."""
     dev = t.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != _current_device():
         raise ValueError(f"{name} must be a CUDA tensor on the current device")
     return dev
 
@@ -162,6 +162,8 @@ def _rows(t, name, dtype, dev):
     """A 2-D tensor whose last dimension is contiguous; returns its row pitch in elements."""
     if t.dtype is not dtype or t.dim() != 2 or t.get_device() != dev:
         raise ValueError(f"{name} must be a 2-D {dtype} tensor on cuda:{dev}")
+    if t.is_contiguous():
+        return t.shape[1]
     n, d = t.shape
     ld, step = t.stride()
     if step != 1 and d > 1:
@@ -181,6 +183,11 @@ def _vec(t, name, shape, dev, dtype=torch.float32):
 
 # the current stream's handle without a Stream object around it (1.3 us less a call)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _current_device():
+    """torch.cuda.current_device() of a process that has a CUDA tensor already."""
+    return torch._C._cuda_getDevice()
 
 
 def _packer(cls):
