@@ -264,7 +264,8 @@ int sj_lora_plan(const int32_t* cu_seqlens_host, int B, const int32_t* ids, int 
  * [N, K], A bf16 [n_adapters, rank, K], Bw bf16 [n_adapters, N, rank], scale
  * fp32 [n_adapters] or NULL (1), bias fp32 [N] or NULL, act as sj_gemm, C bf16
  * with row pitch ldc.  Sums are fp32; scale[a] X A[a]^T is rounded to bf16
- * once on the way into the second product.  plan: the device copy. */
+ * once on the way into the second product.  C overlaps none of the inputs.
+ * plan: the device copy. */
 typedef struct sj_gemm_lora_args {
   const sj_bf16 *X, *W, *A, *Bw;
   const float *scale, *bias;
@@ -288,7 +289,8 @@ int sj_gemm_lora(const sj_gemm_lora_args* args, const sj_lora_plan_info* info,
  *   y  = pre_norm(x')           (skipped when y is NULL)
  * for M rows of D.  post_norm and pre_norm are of `kind`, with weights and
  * optional biases fp32 [D]; y is taken from x' before x' is rounded to x's
- * type.  x_out may be x.  Types are SJ_TYPE_*; pitches are in elements.
+ * type.  x_out may be x itself (with x's pitch); no other output overlaps an input.
+ * Types are SJ_TYPE_*; pitches are in elements.
  * Statistics are fp32. */
 #define SJ_TYPE_F32 0
 #define SJ_TYPE_BF16 1

@@ -17,7 +17,10 @@
 // way.)  Maximum and sum run online in fp32, P is rounded to bf16 as in the tile
 // kernel.  A group whose tiles are many is split into parts, whose maxima, sums
 // and outputs go to the workspace in fp32 and are joined, in order, by a second
-// kernel.  Rows whose output is not finite are computed again over their visible
+// kernel.  Measured: 512 segments of 32 to 512 keys, 4 rows each, 12 heads 107 us
+// (438 MB of K and V: 4.1 TB/s of 6.55; the parts' start and end are short of loads);
+// one row over 60,000 keys 57 us (184 MB: 3.2 TB/s); one segment of 254 rows 9.4 us.
+// Rows whose output is not finite are computed again over their visible
 // keys alone.
 #include <algorithm>
 

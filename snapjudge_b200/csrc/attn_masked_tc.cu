@@ -14,11 +14,17 @@
 // Several such CTAs share an SM (4 at head_dim 64, 2 at 128), so that one's
 // softmax runs beside another's MMAs.  What bounds it is the softmax's
 // instructions (8 to 15 for each score; issue slots about half used).  Measured
-// on 256 x (state + six questions), 12 heads, and on 16 x 2048 with a cap and
-// slopes, 16 heads (us): this form 354 and 762; three chains of 128 threads in
-// one CTA with P in columns of its own, so that MMAs overlap the softmax, 554 and
-// 1,341; two chains with warps of their own for loads, MMAs and work lists, 748
-// and 1,218: fewer softmax warps cost more than the overlap gains.
+// (whole calls): 394 us on 256 x (state of 96 to 400 tokens + six questions) at
+// 12 heads with a bias table (94 us of bytes at 6.55 TB/s, 123 us of exponentials
+// alone); 714 us on 16 x 2048 at 16 heads with a cap and slopes (385 TFLOP/s; cap
+// and exponential alone need 400 us of the two pipes they share); 108 us on 12
+// segments of 701 to 1,499 tokens, 8 heads of 128 over 2, causal, with a cap.
+// Of the first, the same kernel without table 46 us less, without masks 22,
+// without staging the table 26, without the maximum 10.  Other forms, when this
+// one took 354 and 762 on the first two: three chains of 128 threads in one CTA
+// with P in columns of its own, so that MMAs overlap the softmax, 554 and 1,341;
+// two chains with warps of their own for loads, MMAs and work lists, 748 and
+// 1,218: fewer softmax warps cost more than the overlap gains.
 // The reference maximum moves only when a tile's maximum exceeds it by 2^32 (bf16 and
 // fp32 hold such P and sums as exactly as small ones); the row's O in TMEM and its sum
 // are then rescaled.  Sums and O are fp32; P is
@@ -30,7 +36,7 @@
 // the row: a row whose output is not finite is computed again over its visible
 // keys alone (attn_masked_row).
 // At head_dim 128 neither an S buffer for odd tiles (MMAs beside the softmax: 155
-// against 143 us) nor two threads for a row (146) paid.
+// against then 143 us on the third batch above) nor two threads for a row (146) paid.
 // Waits are bounded and failures carried to the next block-wide barrier, as in
 // attn_tc.cu.
 #include <string.h>

@@ -20,6 +20,13 @@
 // launched while the first runs (programmatic dependent launch) and waits for
 // it before its first slab, after all of a tile's k-blocks are on their way.
 // Bounded waits and wind-down as in gemm_tc.cu.
+//
+// What bounds it: the tensor pipe and the epilogue, as the plain GEMM, and the
+// first kernel's pass over X in front.  Measured: 64,500 rows, 768 -> 2304, rank
+// 16 in 48 adapters, 275 us (853 TFLOP/s; sj_gemm without adapters 177 to 188 us);
+// 30,800 rows, 1024 -> 2816, rank 64 in 12, GELU, 212 us (901 TFLOP/s; sj_gemm
+// 140 to 150 us).  The first kernel is 29 us of the former (3.4 TB/s of X); the
+// slabs' MMAs and their loads are the rest.
 #include <algorithm>
 #include <atomic>
 
