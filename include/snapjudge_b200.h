@@ -203,8 +203,9 @@ typedef struct sj_attn_plan_info {
   int32_t longest;   /* key tiles of the longest item */
   int32_t form;      /* SJ_ATTN_* */
   /* few query rows: parts of groups of up to 16 rows, groups of more than one
-   * part, key tiles over all groups, rows of workspace that split groups take */
-  int32_t n_parts, n_splits, n_few_tiles, max_group_rows, ws_rows;
+   * part, key tiles over all groups, rows of workspace that split groups take,
+   * groups, and the parts that one block joins without workspace (0: none) */
+  int32_t n_parts, n_splits, n_few_tiles, max_group_rows, ws_rows, n_groups, join;
   int64_t off_items, off_tiles, off_parts, off_splits, off_few_tiles; /* words into the plan */
 } sj_attn_plan_info;
 

@@ -75,6 +75,7 @@ class AttnPlanInfo(C.Structure):
                 ("n_items", C.c_int32), ("n_tiles", C.c_int32), ("longest", C.c_int32),
                 ("form", C.c_int32), ("n_parts", C.c_int32), ("n_splits", C.c_int32),
                 ("n_few_tiles", C.c_int32), ("max_group_rows", C.c_int32), ("ws_rows", C.c_int32),
+                ("n_groups", C.c_int32), ("join", C.c_int32),
                 ("off_items", _L), ("off_tiles", _L), ("off_parts", _L), ("off_splits", _L),
                 ("off_few_tiles", _L)]
 

@@ -16,12 +16,12 @@
 // (tcgen05 would multiply 128 rows for at most 16; the tensor pipe is idle either
 // way.)  Maximum and sum run online in fp32, P is rounded to bf16 as in the tile
 // kernel.  A group whose tiles are many is split into parts, whose maxima, sums
-// and outputs go to the workspace in fp32 and are joined, in order, by a second
-// kernel.  Measured: 512 segments of 32 to 512 keys, 4 rows each, 12 heads 107 us
+// and outputs are joined in fp32 and in order: by the warps of one block, through
+// shared memory, where a block can hold them all, else through the workspace by a
+// second kernel.  Measured: 512 segments of 32 to 512 keys, 4 rows each, 12 heads 107 us
 // (438 MB of K and V: 4.1 TB/s of 6.55; the parts' start and end are short of loads);
-// one row over 60,000 keys 57 us (184 MB: 3.2 TB/s); one segment of 254 rows 9.4 us.
-// Rows whose output is not finite are computed again over their visible
-// keys alone.
+// one row over 60,000 keys 57 us (184 MB: 3.2 TB/s); one segment of 254 rows 7.3 us.
+// Rows whose output is not finite are computed again over their visible keys alone.
 #include <algorithm>
 
 #include "attn_masked.cuh"
@@ -31,6 +31,7 @@ namespace sjb {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kJoinLd = 68;  // floats of a row in the block's join: 64 dimensions, maximum, sum
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2f(float x) {
@@ -69,25 +70,112 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
+// The block's warps hold parts of the same 16 rows (maximum m, sum l, output o):
+// joined in order, a row by a warp, 64 dimensions at a time.
 template <int DH>
-__global__ void __launch_bounds__(32 * kWarps) attn_few_kernel(const __grid_constant__ AttnMasked p, int mtiles,
-                                                               float* __restrict__ ws) {
+__device__ __forceinline__ void join_block(const AttnMasked& p, int mt, int M, int hk, int row0,
+                                           int warp, const float (&m)[2], const float (&l)[2],
+                                           const float (&o)[DH / 8][4]) {
+  extern __shared__ __align__(16) float part_of[];  // [warps][16][kJoinLd]
+  const int lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3, nw = blockDim.x >> 5;
+  const int G = p.H / p.Hkv;
+#pragma unroll
+  for (int d0 = 0; d0 < DH; d0 += 64) {
+    if (d0) __syncthreads();
+    if (DH == 64 || (c >> 1) == d0 / 64) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float* w = part_of + (warp * 16 + gid + 8 * e) * kJoinLd;
+        if ((c & (DH == 64 ? 3 : 1)) == 0) {
+          w[64] = m[e];
+          w[65] = l[e];
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int t = 0; t < DH / 8; t += 4)
+            *reinterpret_cast<float4*>(w + (2 * c + hh) * (DH / 8) - d0 + t) =
+                make_float4(o[t][2 * e + hh], o[t + 1][2 * e + hh], o[t + 2][2 * e + hh],
+                            o[t + 3][2 * e + hh]);
+      }
+    }
+    __syncthreads();
+    // half a warp for a row, four dimensions a lane
+    const int l4 = 4 * (lane & 15);
+    for (int r0 = 2 * warp; r0 < 16; r0 += 2 * nw) {
+      const int r = r0 + (lane >> 4), q = mt * 16 + r;
+      const float* w = part_of + r * kJoinLd;
+      float mx = -INFINITY;
+      for (int k = 0; k < nw; ++k) mx = fmaxf(mx, w[k * 16 * kJoinLd + 64]);
+      const float mu = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+      for (int k = 0; k < nw; ++k) {
+        const float* wk = w + k * 16 * kJoinLd;
+        const float f = ex2f(wk[64] - mu);
+        const float4 a = *reinterpret_cast<const float4*>(wk + l4);
+        sum += f * wk[65];
+        v[0] += f * a.x, v[1] += f * a.y, v[2] += f * a.z, v[3] += f * a.w;
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] *= inv;
+        odd = odd || !(fabsf(v[i]) <= 3.402823466e38f);
+      }
+      if (q < M)
+        *reinterpret_cast<uint2*>(p.O + (int64_t)(row0 + q / G) * p.ldo +
+                                  (int64_t)(hk * G + q % G) * DH + d0 + l4) =
+            make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+      const unsigned again = __ballot_sync(0xffffffffu, odd && q < M);
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        if (!(again >> (16 * half) & 0xffffu)) continue;
+        const int qh = mt * 16 + r0 + half, row = row0 + qh / G, h = hk * G + qh % G;
+        float x[4];  // dimension lane + 32 i
+        attn_masked_row(p, row, h, lane, x);
+        bf16* out = p.O + (int64_t)row * p.ldo + (int64_t)h * DH + d0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) out[lane + 32 * i] = __float2bfloat16(x[d0 / 32 + i]);
+      }
+    }
+  }
+}
+
+// JOIN: the warps of a block take the parts of one group (p.join at most) and join
+// them through shared memory; else a warp is alone.  (384 threads at 64: 168
+// registers, as without the join; 179 left room for a warp less, 14.6 -> 19.6 us on
+// 64 x 272 keys with one row each.)
+template <int DH, bool JOIN>
+__global__ void __launch_bounds__(JOIN ? (DH == 64 ? 384 : 256) : 32 * kWarps)
+    attn_few_kernel(const __grid_constant__ AttnMasked p, int mtiles, float* __restrict__ ws) {
   constexpr int KC = DH == 64 ? 32 : 16;  // keys at a time
   constexpr int NT = KC / 8;              // S tiles of 8 keys
   constexpr int KL = DH / 32;             // 16-byte loads of a thread for a K row
   constexpr int VL = DH / 64;             // ... for a V row
   constexpr int OT = DH / 8;              // O tiles of 8 columns
   const int lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
-  const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5;
+  const int64_t unit = JOIN ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarps + warp;
   const int hk = (int)(unit % p.Hkv);
   const int64_t rest = unit / p.Hkv;
   const int mt = (int)(rest % mtiles);
-  const int64_t part = rest / mtiles;
-  // the join's blocks may start now; they wait for this kernel's end
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (part >= p.n_parts) return;
-  const int4 pa = p.parts[2 * part], pb = p.parts[2 * part + 1];
-  const int row0 = pa.x, nrows = pa.y, tile0 = pa.z, ntiles = pa.w, ws_row = pb.x;
+  int64_t part = rest / mtiles;
+  int n_own = 1;
+  if constexpr (JOIN) {
+    const int4 gb = p.parts[2 * part + 1];  // the group's first part and parts
+    n_own = gb.z;
+    part = gb.y + min(warp, n_own - 1);
+  } else {
+    // the join's blocks may start now; they wait for this kernel's end
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (part >= p.n_parts) return;
+  }
+  const int4 pa = p.parts[2 * part];
+  const int row0 = pa.x, nrows = pa.y, tile0 = pa.z;
+  const int ntiles = JOIN && warp >= n_own ? 0 : pa.w;
+  const int ws_row = JOIN ? -1 : p.parts[2 * part + 1].x;
   const int G = p.H / p.Hkv, M = nrows * G;
   if (mt * 16 >= M) return;
 
@@ -232,6 +320,13 @@ __global__ void __launch_bounds__(32 * kWarps) attn_few_kernel(const __grid_cons
   // them in o[.][2 e], the second in o[.][2 e + 1]
 #pragma unroll
   for (int e = 0; e < 2; ++e) l[e] = quad_sum(l[e]);
+  if constexpr (JOIN) {
+    if (n_own > 1) {
+      join_block<DH>(p, mt, M, hk, row0, warp, m_ref, l, o);
+      return;
+    }
+    if (warp > 0) return;
+  }
   if (ws_row >= 0) {  // a part: maximum, sum and output for the join
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -351,10 +446,17 @@ __global__ void __launch_bounds__(32 * kWarps) attn_few_join(const __grid_consta
 template <int DH>
 cudaError_t launch(const AttnMasked& p, float* ws, cudaStream_t st) {
   const int mtiles = (std::min(16, p.max_group_rows) * (p.H / p.Hkv) + 15) / 16;
+  if (attn_few_joins(p.join, p.n_groups, p.max_group_rows, p.H, p.Hkv)) {
+    const int64_t blocks = (int64_t)p.n_groups * mtiles * p.Hkv;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    attn_few_kernel<DH, true><<<(unsigned)blocks, 32 * p.join, p.join * 16 * kJoinLd * 4, st>>>(
+        p, mtiles, nullptr);
+    return cudaGetLastError();
+  }
   const int64_t units = (int64_t)p.n_parts * mtiles * p.Hkv;
   const int64_t blocks = (units + kWarps - 1) / kWarps;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  attn_few_kernel<DH><<<(unsigned)blocks, 32 * kWarps, 0, st>>>(p, mtiles, ws);
+  attn_few_kernel<DH, false><<<(unsigned)blocks, 32 * kWarps, 0, st>>>(p, mtiles, ws);
   if (cudaError_t rc = cudaGetLastError()) return rc;
   if (p.n_splits == 0) return cudaSuccess;
   const int64_t jb = ((int64_t)p.n_splits * 16 * p.H + kWarps - 1) / kWarps;

@@ -44,21 +44,25 @@ cudaError_t attn_masked_simt(const AttnMasked& p, cudaStream_t st) {
 }  // namespace sjb
 
 namespace {
+bool few_joins(const sj_attn_plan_info& i, int H, int Hkv) {
+  return sjb::attn_few_joins(i.join, i.n_groups, i.max_group_rows, H, Hkv);
+}
 // Whether the few-row form runs.  The estimates (us) are fits to both forms
 // measured over 22 batches x 3 head shapes (12 and 16 heads of 64; 8 heads of 128
 // over 2 key heads): tiles within 25 %, few rows within 40 %.  Examples,
-// tiles / few: one segment of 254 rows 11 / 9, of 1,024 rows 30 / 41; 512 segments
-// of 272 keys with 4 rows each 229 / 86; one row over 60,000 keys 1,399 / 59.
+// tiles / few: one segment of 254 rows 11 / 7, of 1,024 rows 30 / 42; 512 segments
+// of 272 keys with 4 rows each 232 / 86; one row over 60,000 keys 1,399 / 59.
 //   tiles: the longest item's tiles one after another, slower the more blocks
 //   share an SM, or all tiles at the rate of a full GPU;
-//   few: each tile of a group and key head, and one more launch when groups are split.
+//   few: each tile of a group and key head, and one more launch when
+//   groups are split over blocks.
 bool few_runs(const sj_attn_plan_info& i, int H, int Hkv, int Dh) {
   if ((Dh != 64 && Dh != 128) || i.n_parts == 0 || i.form == SJ_ATTN_TILES) return false;
   if (i.form == SJ_ATTN_FEW) return true;
   const double shared = std::min(3.0, std::max(0.0, (double)i.n_items * H / 148 - 1.0));
   const double tiles = 4.5 + std::max(i.longest * (1.6 + 0.35 * shared), 0.0055 * i.n_tiles * H);
   const int mt = (i.max_group_rows * (H / Hkv) + 15) / 16;
-  const double few = 3.5 + (i.n_splits ? 3.5 : 0.0) +
+  const double few = 3.5 + (i.n_splits && !few_joins(i, H, Hkv) ? 3.5 : 0.0) +
                      0.0027 * (Dh / 64) * mt * Hkv * (double)i.n_few_tiles;
   return few < tiles;
 }
@@ -75,7 +79,7 @@ int64_t sj_attn_masked_workspace(const sj_attn_plan_info* info, int H, int Hkv, 
     bad("bad attention shape");
     return -1;
   }
-  return few_runs(*info, H, Hkv, Dh) ? (int64_t)info->ws_rows * H * (Dh + 4) * 4 : 0;
+  return few_runs(*info, H, Hkv, Dh) && !few_joins(*info, H, Hkv) ? (int64_t)info->ws_rows * H * (Dh + 4) * 4 : 0;
 }
 
 int sj_attn_masked(const sj_attn_masked_args* a, const sj_attn_plan_info* info,

@@ -23,10 +23,21 @@ struct AttnMasked {
   const int32_t* tiles;       // plan: key tiles
   // plan, few query rows (n_parts > 0): 2 x int4 for each part, one for each split
   // group, and the parts' key tiles
-  int n_parts, n_splits, max_group_rows;
+  int n_parts, n_splits, max_group_rows, n_groups, join;
   const int4 *parts, *splits;
   const int32_t* few_tiles;
 };
+
+// Whether the few-row form joins parts inside blocks, `join` warps each, instead
+// of through the workspace and a second kernel.  Measured (us, 12 heads of 64,
+// inside / second kernel): one segment of 254 rows 7.3 / 9.4 (and the call 12 / 18),
+// of 512 rows 11.8 / 16, four of 254 12.3 / 17.4.  Blocks of more than four warps
+// leave an SM's registers half used once there is more than one for each SM: 16 x
+// 2048 keys with 16 rows each, 8 parts, 34 / 26.
+inline bool attn_few_joins(int join, int n_groups, int max_group_rows, int H, int Hkv) {
+  const int64_t mtiles = ((int64_t)max_group_rows * (H / Hkv) + 15) / 16;
+  return join > 0 && (join <= 4 || n_groups * mtiles * Hkv <= 148);
+}
 
 inline AttnMasked attn_masked_params(const sj_attn_masked_args& a, const sj_attn_plan_info& info,
                                      const int32_t* plan) {
@@ -58,6 +69,8 @@ inline AttnMasked attn_masked_params(const sj_attn_masked_args& a, const sj_attn
   p.n_parts = info.n_parts;
   p.n_splits = info.n_splits;
   p.max_group_rows = info.max_group_rows;
+  p.n_groups = info.n_groups;
+  p.join = info.join;
   p.parts = reinterpret_cast<const int4*>(plan + info.off_parts);
   p.splits = reinterpret_cast<const int4*>(plan + info.off_splits);
   p.few_tiles = plan + info.off_few_tiles;

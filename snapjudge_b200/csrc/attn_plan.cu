@@ -15,8 +15,9 @@
 // For few query rows also
 //   parts   8 words each: first row, rows, first key tile, key tiles of a run of a
 //           group's tiles, the workspace row of its first row (-1: the group has
-//           one part), 3 words of padding; a group is up to 16 query rows of one
-//           segment;
+//           one part), and, in the k-th part's words, the k-th group's first part
+//           and number of parts, 1 word of padding; a group is up to 16 query rows
+//           of one segment;
 //   splits  4 words for each group of several parts: first row, rows, parts, first
 //           workspace row;
 //   few     the groups' key tiles, as above.
@@ -41,6 +42,8 @@ struct Iv {
 };
 // Above this many query rows the tile kernel fills the GPU.
 constexpr int kFewMostRows = 4096;
+// Parts that the warps of one block compute and join.
+constexpr int kJoinMost = 8;
 
 // The rows' keys as tiles: `next` tiles greedily over the union of the intervals.
 struct Row {
@@ -168,7 +171,8 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
   std::vector<Part> parts;
   std::vector<std::array<int, 4>> splits;
   std::vector<int32_t> few;
-  int max_rows = 0;
+  std::vector<std::array<int, 2>> first;  // each group's first part and parts
+  int max_rows = 0, join = 0;
   long long ws_rows = 0;
   if (nr > 0 && (p.form == SJ_ATTN_FEW || (p.form == SJ_ATTN_AUTO && nr <= kFewMostRows))) {
     std::vector<Item> groups;
@@ -181,8 +185,11 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
     }
     // parts short enough to spread over the SMs, long enough not to be joined often
     const int most = (int)std::min<long long>(8, 1 + (long long)few.size() * 8 / (148 * 8));
+    int widest = 0;
     for (const Item& g : groups) {
       const int n = std::max(1, (g.tiles + most - 1) / most), per = (g.tiles + n - 1) / n;
+      widest = std::max(widest, n);
+      first.push_back({(int)parts.size(), n});
       max_rows = std::max(max_rows, g.rows);
       if (n > 1) splits.push_back({g.row0, g.rows, n, (int)ws_rows});
       for (int k = 0; k < n; ++k) {
@@ -191,6 +198,9 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
         if (n > 1) ws_rows += g.rows;
       }
     }
+    // at most half of the joining blocks' warps without a part
+    if (widest > 1 && widest <= kJoinMost && (size_t)widest * groups.size() <= 2 * parts.size())
+      join = widest;
   }
 
   if (few.size() > 0x7fffffff || ws_rows > 0x7fffffff) return bad("the batch needs too many key tiles");
@@ -202,6 +212,8 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
   info->off_tiles = info->off_items + 4ll * (long long)items.size();
   info->n_parts = (int)parts.size();
   info->n_splits = (int)splits.size();
+  info->n_groups = (int)first.size();
+  info->join = join;
   info->n_few_tiles = (int)few.size();
   info->longest = items.empty() ? 0 : items[0].tiles;
   info->form = p.form;
@@ -228,7 +240,9 @@ int make_plan(const sj_attn_plan_args& p, int32_t* plan, int64_t plan_len,
   std::fill(plan + info->off_tiles + (long long)tiles.size(), plan + info->off_parts, 0);
   for (size_t k = 0; k < parts.size(); ++k) {
     const Part& q = parts[k];
-    const int32_t v[8] = {q.row0, q.rows, q.tile0, q.tiles, q.ws, 0, 0, 0};
+    const bool g = k < first.size();
+    const int32_t v[8] = {q.row0, q.rows, q.tile0, q.tiles, q.ws, g ? first[k][0] : 0,
+                          g ? first[k][1] : 0, 0};
     std::copy(v, v + 8, plan + info->off_parts + 8 * (long long)k);
   }
   for (size_t k = 0; k < splits.size(); ++k)

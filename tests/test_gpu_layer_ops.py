@@ -324,6 +324,27 @@ def test_attn_python_refusals():
             bad()
 
 
+@pytest.mark.parametrize("H,Hkv,Dh", [(3, 3, 64), (6, 2, 64), (4, 1, 128), (3, 3, 128)])
+@pytest.mark.parametrize("keys,parts", [(130, 2), (150, 3), (250, 4), (370, 6), (500, 8), (700, 11)])
+def test_attn_masked_few_joins(H, Hkv, Dh, keys, parts):
+    """Parts of a group joined in a block (up to 8) or by the second kernel; masked values
+    hold NaN."""
+    m = dict(cu=cum([keys, keys]), q_rows=[3, 11, keys - 1, keys, keys + 40],
+             kv_lens=[keys - 3, keys - 6])
+    plan = plan_of(m, "few")
+    assert plan.info.n_parts == 2 * parts and plan.info.join == (parts if parts <= 8 else 0)
+    g = gen(5)
+    q = rnd((5, H, Dh), g)
+    k, v = rnd((2 * keys, Hkv, Dh), g), rnd((2 * keys, Hkv, Dh), g)
+    ok, _ = sees(m)
+    slopes = 2.0 ** (-8.0 * torch.arange(1, H + 1, device=DEV) / H)
+    want, tol = ref_attn(q, k, v, m, slopes=slopes)
+    clean = ops.attn_masked(q, k, v, plan, slopes=slopes)
+    close(clean, want, tol)
+    v[~ok.any(0)] = math.nan
+    close(ops.attn_masked(q, k, v, plan, slopes=slopes), want, tol)
+
+
 # ---- projection with adapters -------------------------------------------------------
 def ref_lora(x, w, a, b, rows, scale=None, bias=None, act=0):
     x, w, a, b = (t.double() for t in (x, w, a, b))

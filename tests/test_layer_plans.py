@@ -110,6 +110,23 @@ def test_attn_plan_shows_the_defined_keys(case):
     assert (seen == 1).all()
 
 
+@pytest.mark.parametrize("case,join", [
+    (dict(cu=[0, 254]), 4), (dict(cu=[0, 60]), 0), (dict(cu=[0, 60, 188]), 2),
+    (dict(cu=[0, 500], q_rows=[7]), 8), (dict(cu=[0, 600], q_rows=[7]), 0),
+    (dict(cu=[0] + list(range(300, 310)), q_rows=[7, 300, 301, 302, 303, 304]), 0)])
+def test_attn_plan_groups_of_parts(case, join):
+    """Each group's first part and parts stand in the parts' words; a block joins
+    up to 8 of them, where at most half of its warps stay without a part."""
+    rc, info, plan = attn_plan(form=2, **case)
+    assert rc == 0 and info.join == join
+    parts = plan[info.off_parts:info.off_splits].reshape(-1, 8)
+    at = 0
+    for first, n in parts[:info.n_groups, 5:7].tolist():
+        assert first == at and len({tuple(r) for r in parts[first:first + n, :2].tolist()}) == 1
+        at += n
+    assert at == info.n_parts
+
+
 @pytest.mark.parametrize("case", CASES + [dict(cu=[0, 5000], q_rows=[17, 4000])])
 def test_attn_plan_parts_of_few_rows(case):
     """Every query row is in one group, whose parts' tiles cover what it sees,
