@@ -147,8 +147,9 @@ int sj_gemm_lora(const sj_gemm_lora_args* a, const sj_lora_plan_info* info, cons
   p.slabs = reinterpret_cast<const int2*>(plan + info->off_slabs);
   const auto st = static_cast<cudaStream_t>(stream);
   const bool tc = sjb::gemm_lora_tc_supported(p) && !(reinterpret_cast<uintptr_t>(workspace) & 15);
-  const cudaError_t rc =
-      tc ? sjb::gemm_lora_tc(p, workspace, st) : sjb::gemm_lora_simt(p, workspace, st);
+  const cudaError_t rc = !tc                            ? sjb::gemm_lora_simt(p, workspace, st)
+                         : sjb::gemm_lora_small_runs(p) ? sjb::gemm_lora_small(p, st)
+                                                        : sjb::gemm_lora_tc(p, workspace, st);
   if (rc == cudaSuccess) return SJ_OK;
   sjb::set_last_error(std::string("snapjudge CUDA: gemm_lora: ") + cudaGetErrorString(rc));
   return SJ_ERR_CUDA;

@@ -22,6 +22,9 @@ struct GemmLora {
 // tcgen05 kernels (gemm_lora_tc.cu); U: n_slabs / 4 x 256 x 64 bf16 of workspace.
 bool gemm_lora_tc_supported(const GemmLora& p);
 cudaError_t gemm_lora_tc(const GemmLora& p, void* U, cudaStream_t st);
+// One kernel for few rows (gemm_lora_small.cu), same shapes; no workspace.
+bool gemm_lora_small_runs(const GemmLora& p);
+cudaError_t gemm_lora_small(const GemmLora& p, cudaStream_t st);
 // As attn_tc_take_status, for these kernels.
 cudaError_t gemm_lora_take_status(int* code);
 

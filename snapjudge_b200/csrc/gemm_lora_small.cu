@@ -1,0 +1,242 @@
+// gemm_lora_small.cu — C = act(X W^T + bias + scale_a (X A_a^T) B_a^T) for few rows,
+// in one launch.
+//
+// A block computes 16 rows x 32 columns.  Four of its warps split the contraction
+// X W^T over K, the other four, at the same time, that of X A_a^T for up to two
+// slabs (adapter, 16 ranks) of the tile's rows: operands go from global memory
+// (L2) straight into mma.sync m16n8k16, whose sum over K may run in any order, so
+// a thread's 16 bytes of a row are its operand words for two steps.  The partial
+// sums meet in shared memory; then four warps add up 8 columns each, and multiply
+// the tile's U (rounded to bf16, from shared memory) with their rows of B, one slab
+// at a time, adding the product to the rows that use the slab's adapter alone: no
+// value of another adapter reaches a row.  Tiles with more slabs go round again.
+// What bounds it is latency: W is read once for each 16 rows, from L2, and every
+// block computes its rows' U anew, which is why it is for few rows.
+#include <type_traits>
+
+#include "gemm_lora.cuh"
+#include "kernels.h"
+#include "tc_host.h"
+
+namespace sjb {
+namespace {
+
+constexpr int kRows = 16, kCols = 32, kSlabs = 2, kTiles = kCols / 8;
+constexpr int kAccLd = kCols + 4, kULd = 20;  // floats of a row in shared memory
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// acc[t] += x (16 rows) . y[t] (8 rows) over the warp's quarter of K, 32 at a time.
+// x[e], y[t]: this thread's rows, from its first 16 bytes on; y[t] null: zeros.
+template <int NT>
+__device__ __forceinline__ void contract(const bf16* const (&x)[2], const bf16* const (&y)[NT],
+                                         int K, int quarter, int c, float (&acc)[NT][4]) {
+  constexpr int D = NT == 4 ? 3 : 4;  // steps whose loads go out together
+  for (int k0 = 32 * quarter; k0 < K; k0 += 128 * D) {
+    uint4 xv[D][2], yv[D][NT];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int k = k0 + 128 * d;
+      const bool in = k + 8 * c < K;  // K % 8 == 0
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        xv[d][e] = in ? __ldg(reinterpret_cast<const uint4*>(x[e] + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        yv[d][t] = in && y[t] ? __ldg(reinterpret_cast<const uint4*>(y[t] + k))
+                              : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const uint32_t a0[4] = {xv[d][0].x, xv[d][1].x, xv[d][0].y, xv[d][1].y};
+      const uint32_t a1[4] = {xv[d][0].z, xv[d][1].z, xv[d][0].w, xv[d][1].w};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        mma16816(acc[t], a0, yv[d][t].x, yv[d][t].y);
+        mma16816(acc[t], a1, yv[d][t].z, yv[d][t].w);
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256, 2) gemm_lora_small_kernel(const __grid_constant__ GemmLora p) {
+  __shared__ __align__(16) float s_acc[4][kRows][kAccLd];
+  __shared__ __align__(16) float s_u[kSlabs][4][kRows][kULd];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, c = lane & 3;
+  const int m0 = blockIdx.y * kRows, n0 = blockIdx.x * kCols;
+  const int per = (p.R + 15) / 16;  // slabs of an adapter
+
+  // the tile's rows and their adapters: lane r has row r's
+  const int mine = lane < kRows && m0 + lane < p.M ? p.rows[m0 + lane] : -1;
+  const int row[2] = {min(m0 + gid, p.M - 1), min(m0 + gid + 8, p.M - 1)};
+  const bf16* x[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) x[e] = p.X + (int64_t)row[e] * p.ldx + 8 * c;
+  const int own[2] = {__shfl_sync(0xffffffffu, mine, gid), __shfl_sync(0xffffffffu, mine, gid + 8)};
+
+  // rounds of up to kSlabs slabs: all warps walk the same list
+  unsigned todo = __ballot_sync(0xffffffffu, mine >= 0);
+  int slab = 0;  // next slab of the adapter of todo's lowest row
+  float acc[4];
+  const int n = n0 + 8 * warp + gid;  // the row of B of this thread
+  for (bool first = true; first || todo; first = false) {
+    int adapter[kSlabs], rank0[kSlabs];
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s) {
+      adapter[s] = -1;
+      rank0[s] = 0;
+      if (!todo) continue;
+      const int a = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+      adapter[s] = a;
+      rank0[s] = 16 * slab;
+      if (++slab == per) {
+        slab = 0;
+        todo &= ~__ballot_sync(0xffffffffu, mine == a);
+      }
+    }
+    // what the second product needs, on its way before the first ones' loads
+    uint32_t b[kSlabs][2];
+    float scale[kSlabs];
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s) {
+      const bool use = warp < kTiles && adapter[s] >= 0;
+      scale[s] = use && p.scale ? __ldg(p.scale + adapter[s]) : 1.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = rank0[s] + 2 * c + 8 * i;
+        b[s][i] = use && n < p.N && r < p.R
+                      ? __ldg(reinterpret_cast<const unsigned*>(
+                            p.B + ((int64_t)adapter[s] * p.N + n) * p.R + r))
+                      : 0u;
+      }
+    }
+    if (!first) __syncthreads();  // the round before is done with s_u
+    if (first && warp < 4) {
+      float part[kTiles][4] = {};
+      const bf16* w[kTiles];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        w[t] = p.W + (int64_t)min(n0 + 8 * t + gid, p.N - 1) * p.K + 8 * c;
+      contract(x, w, p.K, warp, c, part);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float2*>(&s_acc[warp][gid + 8 * e][8 * t + 2 * c]) =
+              make_float2(part[t][2 * e], part[t][2 * e + 1]);
+    }
+    if (warp >= 4 && adapter[0] >= 0) {
+      auto slabs = [&](auto n_slabs) {
+        constexpr int S = decltype(n_slabs)::value;
+        float u[2 * S][4] = {};
+        const bf16* a[2 * S];
+#pragma unroll
+        for (int t = 0; t < 2 * S; ++t) {
+          const int r = rank0[t >> 1] + 8 * (t & 1) + gid;
+          a[t] = adapter[t >> 1] >= 0 && r < p.R
+                     ? p.A + ((int64_t)adapter[t >> 1] * p.R + r) * p.K + 8 * c
+                     : nullptr;
+        }
+        contract(x, a, p.K, warp - 4, c, u);
+#pragma unroll
+        for (int t = 0; t < 2 * S; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float2*>(
+                &s_u[t >> 1][warp - 4][gid + 8 * e][8 * (t & 1) + 2 * c]) =
+                make_float2(u[t][2 * e], u[t][2 * e + 1]);
+      };
+      if (adapter[1] < 0) slabs(std::integral_constant<int, 1>{});
+      else slabs(std::integral_constant<int, kSlabs>{});
+    }
+    __syncthreads();
+    if (warp >= kTiles) continue;
+    if (first) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float2 v = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 b =
+              *reinterpret_cast<const float2*>(&s_acc[k][gid + 8 * e][8 * warp + 2 * c]);
+          v.x += b.x;
+          v.y += b.y;
+        }
+        acc[2 * e] = v.x;
+        acc[2 * e + 1] = v.y;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s) {
+      if (adapter[s] < 0) continue;
+      uint32_t a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // rows gid and gid + 8, ranks 2 c and 2 c + 8
+        float2 v = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 u = *reinterpret_cast<const float2*>(
+              &s_u[s][k][gid + 8 * (i & 1)][2 * c + 8 * (i >> 1)]);
+          v.x += u.x;
+          v.y += u.y;
+        }
+        a[i] = pack_bf16(v.x * scale[s], v.y * scale[s]);
+      }
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+      mma16816(d, a, b[s][0], b[s][1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (own[e] == adapter[s]) {
+          acc[2 * e] += d[2 * e];
+          acc[2 * e + 1] += d[2 * e + 1];
+        }
+    }
+  }
+
+  const int col = n0 + 8 * warp + 2 * c;  // N % 8 == 0
+  if (warp >= kTiles || col >= p.N) return;
+  const float2 bias =
+      p.bias ? __ldg(reinterpret_cast<const float2*>(p.bias + col)) : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (m0 + gid + 8 * e >= p.M) continue;
+    float v[2] = {acc[2 * e] + bias.x, acc[2 * e + 1] + bias.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (p.act == ACT_GELU) v[i] = gelu_erf(v[i]);
+      else if (p.act == ACT_RELU) v[i] = v[i] < 0.f ? 0.f : v[i];  // a NaN stays one
+    }
+    *reinterpret_cast<uint32_t*>(p.C + (int64_t)(m0 + gid + 8 * e) * p.ldc + col) =
+        pack_bf16(v[0], v[1]);
+  }
+}
+
+}  // namespace
+
+// Up to two blocks an SM, and up to four slabs: by M, one adapter, 768 -> 2304 and
+// 2816 -> 1024 (us on the GPU, this form / tcgen05): 1 4.2 / 10.5 and 8.4 / 19; 37
+// 5.9 / 10.1 and 9.6 / 19; 64 5.9 / 10.1; 96 11.7 / 10.2 and 12.3 / 19; 192 16.9 /
+// 10.4 and 24 / 19.  12 slabs (1024 -> 2816): 16 rows 26 / 14.
+bool gemm_lora_small_runs(const GemmLora& p) {
+  const int64_t rows = ((int64_t)p.M + kRows - 1) / kRows, cols = ((int64_t)p.N + kCols - 1) / kCols;
+  return rows * cols <= 2 * tc::sm_count() && p.max_slabs <= 4;
+}
+
+cudaError_t gemm_lora_small(const GemmLora& p, cudaStream_t st) {
+  gemm_lora_small_kernel<<<dim3((p.N + kCols - 1) / kCols, (p.M + kRows - 1) / kRows), 256, 0,
+                           st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace sjb

@@ -190,6 +190,17 @@ def _current_device():
     return torch._C._cuda_getDevice()
 
 
+# (empty_strided takes 1.6 us, empty with a device 2.4)
+def _out(n, d, like):
+    return torch.empty_strided((n, d), (d, 1), dtype=torch.bfloat16, device=like.device)
+
+
+def _workspace(need, like):
+    if not need:
+        return None
+    return torch.empty_strided((need,), (1,), dtype=torch.uint8, device=like.device)
+
+
 def _packer(cls):
     """A function that lays out a ctypes structure's fields as its bytes (an
     order of magnitude faster than filling the structure)."""
@@ -300,8 +311,7 @@ def attn_masked(q, k, v, plan, *, scale=None, softcap=0.0, rel_bias=None, slopes
         if need < 0:
             check(_lib.SJ_ERR_INVALID)
         plan.workspace[H, Hkv, Dh] = need
-    O = torch.empty((n, H * Dh), dtype=torch.bfloat16, device=q.device)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    O, ws = _out(n, H * Dh, q), _workspace(need, q)
     args = _attn_masked_args(q.data_ptr(), k.data_ptr(), v.data_ptr(), O.data_ptr(), ldq, ldk, ldv,
                              H * Dh, H, Hkv, Dh, Dh ** -0.5 if scale is None else scale, softcap,
                              rel, R, slope)
@@ -357,8 +367,7 @@ def gemm_lora(X, W, A, B, plan, *, scale=None, bias=None, act=0):
     bias_ = _vec(bias, "bias", (N,), dev)
     L = _lib.lib()
     need = plan.workspace
-    C_ = torch.empty((M, N), dtype=torch.bfloat16, device=X.device)
-    ws = torch.empty(need, dtype=torch.uint8, device=X.device) if need else None
+    C_, ws = _out(M, N, X), _workspace(need, X)
     args = _gemm_lora_args(X.data_ptr(), w, a, b, s, bias_, C_.data_ptr(), ldx, N, N, K, act)
     rc = L.sj_gemm_lora(args, plan.info_ref, plan.data.data_ptr(), _at(ws), need, _raw_stream(dev))
     if rc:

@@ -404,6 +404,29 @@ def test_lora(lens, ids, n, N, K, R, act, biased, scaled):
     close(got, *ref_lora(t["x"], t["w"], t["a"], t["b"], rows, act=act, **kw))
 
 
+@pytest.mark.parametrize("lens,ids,n,N,K,R", [
+    ([1] * 21, [0, 2, -1, 1, 3, 0, 0] * 3, 4, 72, 264, 8),  # adapters that change with every row
+    ([17, 15, 1], [0, -1, 1], 2, 768, 8, 16),               # K below one step of a warp
+    ([3, 30], [1, 0], 2, 40, 1000, 24),                     # two slabs an adapter, N within a tile
+    ([16], [0], 1, 2304, 768, 64),                          # two rounds of slabs
+    ([64], [0], 1, 2304, 768, 16),                          # the most rows in one launch there
+    ([65], [0], 1, 2304, 768, 16),                          # ... and one more
+    ([12, 12], [1, 0], 2, 64, 64, 40),                      # more slabs than one launch takes
+])
+def test_lora_few_rows(lens, ids, n, N, K, R):
+    cu = cum(lens)
+    t, kw, rows, plan = lora_inputs(cu, ids, N, K, R, n, 27, biased=True)
+    want, tol = ref_lora(t["x"], t["w"], t["a"], t["b"], rows, act=1, **kw)
+    close(ops.gemm_lora(t["x"], t["w"], t["a"], t["b"], plan, act=1, **kw), want, tol)
+    for name in ("a", "b"):  # a spoilt adapter stays with its rows
+        s = dict(t)
+        s[name] = t[name].clone()
+        s[name][0] = math.nan
+        got = ops.gemm_lora(s["x"], s["w"], s["a"], s["b"], plan, act=1, **kw)
+        close(got[rows != 0], want[rows != 0], tol[rows != 0])
+        assert not torch.isfinite(got[rows == 0]).any()
+
+
 @pytest.mark.parametrize("lens", [[40, 200, 60], [900, 900, 900]])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 def test_lora_a_spoilt_adapter_stays_with_its_rows(lens, value):
