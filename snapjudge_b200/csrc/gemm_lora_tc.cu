@@ -24,7 +24,7 @@
 // What bounds it: the tensor pipe and the epilogue, as the plain GEMM, and the
 // first kernel's pass over X in front.  Measured: 64,500 rows, 768 -> 2304, rank
 // 16 in 48 adapters, 275 us (853 TFLOP/s; sj_gemm without adapters 177 to 188 us);
-// 30,800 rows, 1024 -> 2816, rank 64 in 12, GELU, 212 us (901 TFLOP/s; sj_gemm
+// 30,800 rows, 1024 -> 2816, rank 64 in 12, GELU, 209 us (914 TFLOP/s; sj_gemm
 // 140 to 150 us).  The first kernel is 29 us of the former (3.4 TB/s of X); the
 // slabs' MMAs and their loads are the rest.
 #include <algorithm>
@@ -206,44 +206,54 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// ---- U by rows, for blocks of many adapters: one warp a row -----------------------
+// ---- U by rows, for blocks of many adapters: one warp for a row and 8 ranks ---------
 // U[row, r] = scale_a X[row] . A_a[r], rounded to bf16
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
     lora_shrink_rows_kernel(const __grid_constant__ GemmLora p, bf16* __restrict__ U) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int64_t row = unit / (p.R / 8);  // R is a multiple of 8
   if (row >= p.M) return;
+  const int r0 = 8 * (int)(unit % (p.R / 8));
   const int a = p.rows[row];
   if (a < 0) return;  // its U is not read
   const float f = p.scale ? p.scale[a] : 1.f;
   const bf16* x = p.X + row * p.ldx;
   const bf16* ar = p.A + (int64_t)a * p.R * p.K;
-  for (int r0 = 0; r0 < p.R; r0 += 8) {  // R is a multiple of 8
-    float acc[8] = {};
-    for (int k = 8 * lane; k < p.K; k += 256) {  // and K
-      const uint4 xv = *reinterpret_cast<const uint4*>(x + k);
-      uint4 av[8];
+  float acc[8] = {};
+  for (int k0 = 8 * lane; k0 < p.K; k0 += 256 * 3) {  // and K; 27 loads together
+    uint4 xv[3], av[3][8];
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+      const int k = k0 + 256 * d;
+      const bool in = k < p.K;
+      xv[d] = in ? __ldg(reinterpret_cast<const uint4*>(x + k)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int r = 0; r < 8; ++r)
-        av[r] = *reinterpret_cast<const uint4*>(ar + (int64_t)(r0 + r) * p.K + k);
-#pragma unroll
-      for (int r = 0; r < 8; ++r) acc[r] += dot8(xv, av[r]);
+        av[d][r] = in ? __ldg(reinterpret_cast<const uint4*>(ar + (int64_t)(r0 + r) * p.K + k))
+                      : make_uint4(0, 0, 0, 0);
     }
-    float mine = 0.f;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const float t = warp_sum(acc[r]);
-      mine = lane == r ? t : mine;
-    }
-    if (lane < 8) U[row * p.R + r0 + lane] = __float2bfloat16(f * mine);
+    for (int d = 0; d < 3; ++d)
+#pragma unroll
+      for (int r = 0; r < 8; ++r) acc[r] += dot8(xv[d], av[d][r]);
   }
+  float mine = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float t = warp_sum(acc[r]);
+    mine = lane == r ? t : mine;
+  }
+  if (lane < 8) U[row * p.R + r0 + lane] = __float2bfloat16(f * mine);
 }
 
 // ---- the GEMM -----------------------------------------------------------------------
-// GATHER: no slabs; the epilogue adds U[row] . B_a[n], its own adapter's alone, from
-// memory.  For tiles of few columns whose rows use many adapters: 600 rows with 64
-// adapters of rank 8, 768 x 768: 58 slabs in a block.
+// GATHER: no slabs; while a tile is computed, its epilogue warps work out U[row] .
+// B_a[n] with each row's own adapter and add it to the accumulators.  For tiles of few
+// columns whose rows use many adapters: 600 rows with 64 adapters of rank 8, 768 ->
+// 768, 11.4 us on the GPU (7.8 without adapters; 16.1 with a thread for each row
+// reading its B alone, after the tile); 32 ranks 24 (47).
 template <int BN, bool PAIR>
 struct Cfg {
   static constexpr int kEpiWarps = BN >= 64 ? 8 : 4;
@@ -343,21 +353,31 @@ __device__ __forceinline__ void finish32(const GemmLora& p, const uint32_t (&r)[
   }
 }
 
-// r[j] += U[row] . B_a[n0 + j] for the row's own adapter
-__device__ __forceinline__ void add_own(const GemmLora& p, const bf16* U, int64_t row, int n0,
-                                        uint32_t (&r)[32]) {
-  const int a = p.rows[row];
-  if (a < 0) return;
-  const bf16* b = p.B + ((int64_t)a * p.N + n0) * p.R;
-  for (int r0 = 0; r0 < p.R; r0 += 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(U + row * p.R + r0);
+// out[r][n ^ r] = U[row0 + r] . B_a[n], a = the row's adapter (lane r holds it as
+// `own`), for 32 rows r and this lane's column n
+__device__ __forceinline__ void own_products(const GemmLora& p, const bf16* U, int64_t row0, int n,
+                                             int own, int lane, float (&out)[32][32]) {
+#pragma unroll 1
+  for (int g = 0; g < 32; g += 8) {
+    float d[8] = {};
+    for (int r0 = 0; r0 < p.R; r0 += 8) {
+      uint4 u[8], b[8];
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n0 + j < p.N)
-        r[j] = __float_as_uint(
-            __uint_as_float(r[j]) +
-            dot8(u, __ldg(reinterpret_cast<const uint4*>(b + (int64_t)j * p.R + r0))));
+      for (int i = 0; i < 8; ++i) {
+        const int a = __shfl_sync(0xffffffffu, own, g + i);
+        const bool in = a >= 0 && n < p.N;
+        u[i] = in ? __ldcg(reinterpret_cast<const uint4*>(U + (row0 + g + i) * p.R + r0))
+                  : make_uint4(0, 0, 0, 0);
+        b[i] = in ? __ldg(reinterpret_cast<const uint4*>(p.B + ((int64_t)a * p.N + n) * p.R + r0))
+                  : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] += dot8(u[i], b[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[g + i][lane ^ (g + i)] = d[i];
   }
+  __syncwarp();
 }
 
 template <int BN, bool PAIR, bool GATHER>
@@ -373,6 +393,8 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
   constexpr uint32_t IDESC = idesc_bf16(F::kTileM, BN, false, false);
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], tfull_bar[2], tempty_bar[2], drain_bar;
+  static_assert(!GATHER || 32 * F::kEpiWarps / 4 == BN, "32 columns a warp");
+  __shared__ float own_sh[GATHER ? F::kEpiWarps : 1][GATHER ? 32 : 1][GATHER ? 32 : 1];
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_sh;
 
@@ -560,7 +582,6 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
     constexpr int PARTS = F::kEpiWarps / 4;  // warps of a row quarter share its columns
-    if constexpr (GATHER) pdl_wait();        // U, read by the epilogue
     const int q = warp & 3, hf = (warp - 2) >> 2;
     uint8_t* stg = smem + STAGES * F::kStageBytes + (warp - 2) * 2 * 32 * 128;
     int sbuf = 0, local = 0;
@@ -575,6 +596,15 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
       const int row0 = (t / n_tiles) * F::kTileM + (int)rank * BM + q * 32;
       const int64_t row = row0 + lane;
       const int col0 = (t % n_tiles) * BN;
+      int own = -1;
+      if constexpr (GATHER) {
+        // while the tile is computed: every row's U . B of its adapter, lane = column,
+        // row by row (whole lines of B), kept for the rows' threads in shared memory
+        own = row < p.M ? p.rows[row] : -1;
+        if (local == 0) pdl_wait();  // U
+        __syncwarp();                // the tile before is done with its products
+        own_products(p, U, row0, col0 + hf * 32 + lane, own, lane, own_sh[warp - 2]);
+      }
       int ok = 1;
       if (lane == 0) ok = mbar_wait<true>(&tfull_bar[b], (local >> 1) & 1) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -625,7 +655,11 @@ __global__ void __launch_bounds__(Cfg<BN, PAIR>::kThreads, 1)
           tmem_ld32(tacc + c, r);
           tmem_ld_wait();
           if (row >= p.M) continue;
-          if constexpr (GATHER) add_own(p, U, row, col0 + c, r);
+          if constexpr (GATHER) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              r[j] = __float_as_uint(__uint_as_float(r[j]) + own_sh[warp - 2][lane][j ^ lane]);
+          }
           float v[32];
           finish32(p, r, row, col0 + c, check, v);
           bf16* out = p.C + row * p.ldc + col0 + c;
@@ -758,16 +792,20 @@ cudaError_t gemm_lora_tc(const GemmLora& p, void* U, cudaStream_t st) {
   const int64_t mt = (p.M + BM - 1) / BM;
   const int sms = sm_count();
   const bool pair = p.M >= 2048;
+  // Tiles pay for each slab, the gather for each rank of each column.  512 rows, 768
+  // -> 768 (us, gather / slabs): rank 8, 5 slabs 11.2 / 13.9, 48 11.5 / 26; rank 16, 8
+  // slabs 14.8 / 17; rank 32, 32 slabs 23 / 19, 64 23 / 25; rank 64, 128 slabs 48 / 35.
+  const bool many = p.max_slabs > 4 && 24ll * p.max_slabs > (int64_t)p.R * p.R;
   const int bn = pair                                   ? 256
                  : mt * ((p.N + 255) / 256) >= sms      ? 256
                  : mt * ((p.N + 127) / 128) >= sms      ? 128
                  : mt * ((p.N + 63) / 64) >= sms        ? 64
                                                         : 32;
-  // tiles of few columns pay about 100 cycles for each slab, and 4 x rank for each
-  // column of the gather
-  const bool gather = bn <= 64 && 10 * p.max_slabs > 13 * p.R;
+  const bool gather = bn <= 64 && many;
   if (gather) {
-    lora_shrink_rows_kernel<<<(unsigned)((p.M + 7) / 8), 256, 0, st>>>(p, u);
+    const int64_t units = (int64_t)p.M * (p.R / 8);
+    if (units > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    lora_shrink_rows_kernel<<<(unsigned)((units + 3) / 4), 128, 0, st>>>(p, u);
     if (cudaError_t rc = cudaGetLastError()) return rc;
     return bn == 64 ? launch_gemm<64, false, true>(p, mx, u, st)
                     : launch_gemm<32, false, true>(p, mx, u, st);
